@@ -447,8 +447,8 @@ def _plain_tables(st):
     slots = torch.where((t < tok[-1:]) & ok, block * bs + pos % bs, -1)
     live = (new >= 0).long()
     return _tables_out(table, torch.where(ok, need * live, held).int(),
-                       torch.where(ok, after * live, lens).int(), free, left.int(), slots, tok.int(),
-                       status.int())
+                       torch.where(ok, after * live, lens).int(), free, left.int(), slots,
+                       torch.where(ok, tok, 0).int(), status.int())
 
 
 _PLAIN = {"decode": _plain_decode, "prefill": _plain_prefill, "tables": _plain_tables}
