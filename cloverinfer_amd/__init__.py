@@ -14,7 +14,10 @@ _EXPORTS = {
     "GpuAttentionBackend": "attention_backend",
     "create_attention_backend": "attention_backend",
     "KVCacheManager": "memory_manager",
+    "advance_block_tables": "kernels",
     "chunked_prefill": "kernels",
+    "differential_attention": "kernels",
+    "differential_prefill": "kernels",
     "paged_attention": "kernels",
     "reshape_and_cache": "kernels",
 }

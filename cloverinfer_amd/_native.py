@@ -116,6 +116,45 @@ class PrefillArgs(ctypes.Structure):
     ]
 
 
+class DiffArgs(ctypes.Structure):
+    """Mirror of ``clv_diff_args``."""
+
+    _fields_ = [
+        ("lambda_", _c_ptr),
+        ("lambda_stride_row", _c_i64),
+        ("lambda_stride_head", _c_i64),
+        ("norm_weight", _c_ptr),
+        ("lambda_value", ctypes.c_float),
+        ("norm_eps", ctypes.c_float),
+        ("out_scale", ctypes.c_float),
+    ]
+
+
+class TablesArgs(ctypes.Structure):
+    """Mirror of ``clv_tables_args``."""
+
+    _fields_ = [
+        ("block_tables", _c_ptr),
+        ("blocks_held", _c_ptr),
+        ("context_lens", _c_ptr),
+        ("new_lens", _c_ptr),
+        ("free_blocks", _c_ptr),
+        ("num_free", _c_ptr),
+        ("blocks_held_out", _c_ptr),
+        ("context_lens_out", _c_ptr),
+        ("num_free_out", _c_ptr),
+        ("slot_mapping", _c_ptr),
+        ("query_start_loc", _c_ptr),
+        ("status", _c_ptr),
+        ("num_tokens", _c_i64),
+        ("rows", _c_i32),
+        ("width", _c_i32),
+        ("block_size", _c_i32),
+        ("num_blocks", _c_i32),
+        ("reserve", _c_i32),
+    ]
+
+
 # Exported symbols and their (restype, argtypes).
 SIGNATURES = {
     "clv_abi_version": (ctypes.c_int, []),
@@ -178,6 +217,23 @@ SIGNATURES = {
     "clv_chunked_prefill_split": (ctypes.c_int, [ctypes.POINTER(PrefillArgs), _c_ptr,
                                                  ctypes.c_size_t, _c_ptr]),
     "clv_prefill_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PrefillArgs)]),
+    "clv_diff_decode": (
+        ctypes.c_int,
+        [ctypes.POINTER(DecodeArgs), ctypes.POINTER(DiffArgs), _c_ptr, _c_ptr, _c_i32, _c_ptr,
+         ctypes.c_size_t, _c_ptr],
+    ),
+    "clv_diff_decode_workspace_bytes": (
+        ctypes.c_size_t, [ctypes.POINTER(DecodeArgs), _c_i32, _c_i32],
+    ),
+    "clv_diff_prefill": (
+        ctypes.c_int,
+        [ctypes.POINTER(PrefillArgs), ctypes.POINTER(DiffArgs), _c_ptr, ctypes.c_size_t, _c_ptr],
+    ),
+    "clv_diff_prefill_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PrefillArgs)]),
+    "clv_advance_block_tables": (
+        ctypes.c_int, [ctypes.POINTER(TablesArgs), _c_ptr, ctypes.c_size_t, _c_ptr],
+    ),
+    "clv_tables_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(TablesArgs)]),
 }
 
 _lock = threading.Lock()

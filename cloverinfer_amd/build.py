@@ -43,6 +43,7 @@ SOURCES = [
     "prefill.hip",
     "prefill_f32.hip",
     "prefill_mfma.hip",
+    "tables.hip",
 ]
 
 ARCH = "gfx950"

@@ -106,13 +106,86 @@ __device__ __forceinline__ void merge_and_store(const WaveSmem<NW, GR, D> &sm, i
   }
 }
 
+// Lambda of (row of q, query head).
+__device__ __forceinline__ float diff_lambda(const DiffParams &d, int64_t row, int head) {
+  return d.lam != nullptr ? d.lam[row * d.lam_row + head * d.lam_head] : d.lam_value;
+}
+
+// Factor of a differential row before its norm weight, from the sum of its
+// squares.
+__device__ __forceinline__ float diff_factor(const DiffParams &d, float sum_sq, int dim) {
+  return d.weight != nullptr ? d.out_scale * rsqrtf(sum_sq / (float)dim + d.eps) : d.out_scale;
+}
+
+// merge_and_store for differential rows: rows 2i and 2i + 1 of the workgroup
+// are the two maps of its i-th query head (0 <= i < ng / 2), written at
+// out + i * out_stride; qrow and head0 name the row of q and the first query
+// head (for lambda). D / 8 lanes share a row, and sum its squares among them.
+template <typename T, int NW, int GR, int D>
+__device__ __forceinline__ void diff_merge_and_store(const WaveSmem<NW, GR, D> &sm, int ng,
+                                                     const DiffParams &d, int64_t qrow, int head0,
+                                                     T *out, int64_t out_stride) {
+  constexpr int CPR = D / 8;
+  for (int idx = threadIdx.x; idx < GR / 2 * CPR; idx += NW * 64) {
+    const int i = idx / CPR;
+    const int c = idx - i * CPR;
+    if (2 * i >= ng) continue;
+    float acc[2][8];
+#pragma unroll
+    for (int map = 0; map < 2; ++map) {
+      const int g = 2 * i + map;
+      float M = kNegInf;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, sm.m[w][g]);
+      const float Msub = (M == kNegInf) ? 0.f : M;
+      float L = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[map][e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float wt = fast_exp2(sm.m[w][g] - Msub);
+        L += sm.l[w][g] * wt;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[map][e] += sm.o[w][g][c * 8 + e] * wt;
+      }
+      const float inv = L > 0.f ? 1.f / L : 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[map][e] *= inv;
+    }
+    const float lam = diff_lambda(d, qrow, head0 + i);
+    float o[8], ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      o[e] = acc[0][e] - lam * acc[1][e];
+      ss += o[e] * o[e];
+    }
+#pragma unroll
+    for (int off = 1; off < CPR; off <<= 1) ss += shfl_xor(ss, off);
+    const float f = diff_factor(d, ss, D);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= d.weight != nullptr ? f * d.weight[c * 8 + e] : f;
+    T *dst = out + (int64_t)i * out_stride + c * 8;
+    if constexpr (sizeof(T) == 2) {
+      uint32_t r[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[e] = __builtin_bit_cast(uint16_t, (T)o[e]);
+      store_vec<u32x4>(dst, (u32x4){r[0] | (r[1] << 16), r[2] | (r[3] << 16), r[4] | (r[5] << 16),
+                                    r[6] | (r[7] << 16)});
+    } else {
+      store_vec<f32x4>(dst, (f32x4){o[0], o[1], o[2], o[3]});
+      store_vec<f32x4>(dst + 4, (f32x4){o[4], o[5], o[6], o[7]});
+    }
+  }
+}
+
 // VALU attention of ng (<= GM) query rows over tokens [t_begin, t_end) of
 // one kv head; leaves each wave's partial in sm (caller syncs and merges).
 // Lane layout: a token row of D elements is split into 16-byte chunks, LPT
 // lanes per token, TPI tokens per wave iteration. Each lane keeps its own
 // online-softmax state per query row; the TPI token rows are merged at the
-// end with the log-sum-exp rule.
-template <typename T, int D, int GM, int NW>
+// end with the log-sum-exp rule. DIFF: rows 2i and 2i + 1 are the two maps of
+// query row i, each one half of q with zeros in the other.
+template <typename T, int D, int GM, int NW, bool DIFF = false>
 __device__ __forceinline__ void valu_attend(const T *q0, int64_t q_stride_head, int ng,
                                             const KvView &kv, int t_begin, int t_end,
                                             float scale_log2, WaveSmem<NW, GM, D> &sm) {
@@ -130,10 +203,12 @@ __device__ __forceinline__ void valu_attend(const T *q0, int64_t q_stride_head, 
 #pragma unroll
   for (int g = 0; g < GM; ++g) {
     if (g < ng) {
-      const u32x4 w = load_vec<u32x4>(q0 + (int64_t)g * q_stride_head + col * VEC);
+      const u32x4 w =
+          load_vec<u32x4>(q0 + (int64_t)(DIFF ? g / 2 : g) * q_stride_head + col * VEC);
       const T *e = (const T *)&w;
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) qf[g][v] = to_f32(e[v]);
+      for (int v = 0; v < VEC; ++v)
+        qf[g][v] = !DIFF || (col * VEC + v >= D / 2) == (g % 2 == 1) ? to_f32(e[v]) : 0.f;
     } else {
 #pragma unroll
       for (int v = 0; v < VEC; ++v) qf[g][v] = 0.f;

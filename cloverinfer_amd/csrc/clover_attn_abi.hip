@@ -464,16 +464,19 @@ int head_group(int num_kv_heads, int num_waves) {
   return std::max(hg, 1);
 }
 
-// Validates a balanced-decode call and lays the workspace out in p.
+// Validates a balanced-decode call and lays the workspace out in p. diff: a
+// differential decode, `a` counting the rows of both maps as heads.
 int fill_balanced(const clv_decode_args *a, int32_t num_waves, void *workspace,
-                  size_t workspace_bytes, clv::DecodeParams *p) {
+                  size_t workspace_bytes, clv::DecodeParams *p, bool diff = false) {
   const int st = fill_decode(a, p);
   if (st != CLV_OK) return st;
   if (num_waves <= 0) num_waves = clv_default_num_waves();
   if (num_waves > (1 << 22)) return CLV_EINVAL;
   const int64_t nseg = (int64_t)p->num_seqs * p->num_kv_heads * p->n_gchunks;
   const int hg = head_group(p->num_kv_heads, num_waves);
-  if (!clv::decode_stream_supported((DType)a->dtype, a->head_dim, a->block_size, nseg))
+  if (diff ? !clv::diff_decode_mfma_supported(a->head_dim, a->block_size) ||
+                 nseg > clv::kStreamMaxSegments
+           : !clv::decode_stream_supported((DType)a->dtype, a->head_dim, a->block_size, nseg))
     return CLV_EUNSUPPORTED;
   if (p->num_seqs == 0) return CLV_OK;
   const size_t need = clv_balanced_workspace_bytes(a->num_seqs, a->num_heads, a->num_kv_heads,
@@ -804,6 +807,169 @@ int clv_chunked_prefill_split(const clv_prefill_args *a, void *workspace, size_t
   ws += round256(rows * 4);
   sp.ws_o = (float *)ws;
   return launch_prefill(p, dt, k, &sp, (hipStream_t)stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+int fill_diff(const clv_diff_args *d, clv::DiffParams *out) {
+  if (d == nullptr) return CLV_EINVAL;
+  if (!isfinite(d->out_scale)) return CLV_EINVAL;
+  if (d->lambda == nullptr && !isfinite(d->lambda_value)) return CLV_EINVAL;
+  if (d->norm_weight != nullptr && !(isfinite(d->norm_eps) && d->norm_eps >= 0.f)) return CLV_EINVAL;
+  *out = clv::DiffParams{d->lambda, d->lambda_stride_row, d->lambda_stride_head, d->lambda_value,
+                         d->norm_weight, d->norm_eps, d->out_scale};
+  return CLV_OK;
+}
+
+// `a` with the rows of both maps as its heads.
+int diff_rows(const clv_decode_args *a, clv_decode_args *rows) {
+  if (a == nullptr || a->num_heads <= 0 || a->num_heads > (1 << 20) || a->num_kv_heads <= 0 ||
+      a->num_heads % a->num_kv_heads != 0)
+    return CLV_EINVAL;
+  *rows = *a;
+  rows->num_heads = 2 * a->num_heads;
+  return CLV_OK;
+}
+
+// Longest context for which a differential decode runs as one launch, a
+// workgroup per (sequence, kv head, 16 rows), where the caller names no wave
+// count (kernels.choose_schedule has the same bound for plain decode).
+constexpr int32_t kDiffSinglePassMaxLen = 512;
+
+bool diff_single_pass(const clv_decode_args &rows, bool fp8, int32_t num_waves) {
+  if (fp8) return false;
+  if (!clv::diff_decode_mfma_supported(rows.head_dim, rows.block_size)) return true;
+  if (num_waves <= 0 && rows.max_context_len <= kDiffSinglePassMaxLen) return true;
+  // More segments than the balanced decode takes: a workgroup each fills the chip.
+  return (int64_t)rows.num_seqs * rows.num_kv_heads *
+             ceil_div(rows.num_heads / rows.num_kv_heads, 16) > clv::kStreamMaxSegments;
+}
+
+int32_t diff_waves(bool fp8, int32_t num_waves) {
+  return num_waves > 0 ? num_waves : fp8 ? clv_default_num_waves_fp8() : clv_default_num_waves();
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t clv_diff_decode_workspace_bytes(const clv_decode_args *a, int32_t fp8, int32_t num_waves) {
+  clv_decode_args r;
+  if (diff_rows(a, &r) != CLV_OK || diff_single_pass(r, fp8 != 0, num_waves)) return 0;
+  return clv_balanced_workspace_bytes(r.num_seqs, r.num_heads, r.num_kv_heads, r.head_dim,
+                                      diff_waves(fp8 != 0, num_waves));
+}
+
+int clv_diff_decode(const clv_decode_args *a, const clv_diff_args *d, const float *k_scales,
+                    const float *v_scales, int32_t num_waves, void *workspace,
+                    size_t workspace_bytes, clv_stream_t stream) {
+  clv_decode_args r;
+  clv::DiffParams diff;
+  int st = diff_rows(a, &r);
+  if (st == CLV_OK) st = fill_diff(d, &diff);
+  if (st != CLV_OK) return st;
+  if ((k_scales == nullptr) != (v_scales == nullptr)) return CLV_EINVAL;
+  const bool fp8 = k_scales != nullptr;
+  if (fp8) {
+    if (a->dtype != CLV_F16 && a->dtype != CLV_BF16) return CLV_EINVAL;
+    if (a->head_dim != 128 || a->block_size < 16) return CLV_EUNSUPPORTED;
+    if ((a->kv_stride_block & 15) || (a->kv_stride_token & 15) || (a->kv_stride_head & 15))
+      return CLV_EINVAL;
+  }
+  const hipStream_t s = (hipStream_t)stream;
+  const DType dt = (DType)a->dtype;
+  clv::DecodeParams p;
+  if (diff_single_pass(r, fp8, num_waves)) {
+    st = fill_decode(&r, &p);
+    if (st != CLV_OK || p.num_seqs == 0) return st;
+    if ((int64_t)p.num_kv_heads * p.n_gchunks > 65535) return CLV_EUNSUPPORTED;  // grid y limit
+    p.diff = diff;
+    const hipError_t err = clv::diff_decode_mfma_supported(a->head_dim, a->block_size)
+                               ? clv::launch_diff_decode_mfma(p, dt, s)
+                               : clv::launch_diff_decode_valu(p, dt, s);
+    return err == hipSuccess ? CLV_OK : CLV_ELAUNCH;
+  }
+  st = fill_balanced(&r, diff_waves(fp8, num_waves), workspace, workspace_bytes, &p, true);
+  if (st != CLV_OK || p.num_seqs == 0) return st;
+  p.diff = diff;
+  if (fp8) {
+    p.kv_fp8 = 1;
+    p.k_scales = k_scales;
+    p.v_scales = v_scales;
+  }
+  if (clv::launch_diff_decode_stream(p, dt, s) != hipSuccess) return CLV_ELAUNCH;
+  return clv::launch_diff_stream_reduce(p, dt, s) == hipSuccess ? CLV_OK : CLV_ELAUNCH;
+}
+
+size_t clv_diff_prefill_workspace_bytes(const clv_prefill_args *a) {
+  (void)a;
+  return 0;
+}
+
+int clv_diff_prefill(const clv_prefill_args *a, const clv_diff_args *d, void *workspace,
+                     size_t workspace_bytes, clv_stream_t stream) {
+  (void)workspace;
+  (void)workspace_bytes;
+  clv::PrefillParams p;
+  clv::DiffParams diff;
+  int st = fill_prefill(a, &p);
+  if (st == CLV_OK) st = fill_diff(d, &diff);
+  if (st != CLV_OK || p.num_seqs == 0 || p.num_tokens == 0) return st;
+  p.diff = diff;
+  p.group *= 2;  // rows of both maps
+  return clv::launch_diff_prefill_valu(p, (DType)a->dtype, (hipStream_t)stream) == hipSuccess
+             ? CLV_OK
+             : CLV_ELAUNCH;
+}
+
+}  // extern "C"
+
+namespace {
+
+// Validates a step of the block tables. An empty table (no rows) is valid.
+int fill_tables(const clv_tables_args *a, clv::TablesParams *p) {
+  if (a == nullptr) return CLV_EINVAL;
+  if (a->rows < 0 || a->width < 0 || a->num_blocks < 0 || a->num_tokens < 0 || a->reserve < 0)
+    return CLV_EINVAL;
+  if (a->num_tokens > INT32_MAX) return CLV_EINVAL;
+  if (!is_pow2(a->block_size) || a->rows > CLV_TABLES_MAX_ROWS) return CLV_EUNSUPPORTED;
+  if ((int64_t)a->width * a->block_size > INT32_MAX) return CLV_EINVAL;
+  if (!a->num_free || !a->num_free_out || !a->query_start_loc || !a->status) return CLV_EINVAL;
+  if (a->num_blocks > 0 && !a->free_blocks) return CLV_EINVAL;
+  if (a->num_tokens > 0 && !a->slot_mapping) return CLV_EINVAL;
+  if (a->rows > 0 && (!a->blocks_held || !a->context_lens || !a->new_lens || !a->blocks_held_out ||
+                      !a->context_lens_out || (a->width > 0 && !a->block_tables)))
+    return CLV_EINVAL;
+  *p = clv::TablesParams{a->block_tables,     a->blocks_held,      a->context_lens,
+                         a->new_lens,         a->free_blocks,      a->num_free,
+                         a->blocks_held_out,  a->context_lens_out, a->num_free_out,
+                         a->slot_mapping,     a->query_start_loc,  a->status,
+                         a->num_tokens,       a->rows,             a->width,
+                         log2_int(a->block_size), a->num_blocks,   a->reserve};
+  return CLV_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t clv_tables_workspace_bytes(const clv_tables_args *a) {
+  clv::TablesParams p;
+  return fill_tables(a, &p) == CLV_OK ? clv::tables_workspace_bytes(p) : 0;
+}
+
+int clv_advance_block_tables(const clv_tables_args *a, void *workspace, size_t workspace_bytes,
+                             clv_stream_t stream) {
+  clv::TablesParams p;
+  const int st = fill_tables(a, &p);
+  if (st != CLV_OK) return st;
+  const size_t need = clv::tables_workspace_bytes(p);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 255u)))
+    return CLV_EWORKSPACE;
+  return clv::launch_tables(p, workspace, (hipStream_t)stream) == hipSuccess ? CLV_OK
+                                                                             : CLV_ELAUNCH;
 }
 
 }  // extern "C"

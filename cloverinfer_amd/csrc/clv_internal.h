@@ -7,7 +7,19 @@
 
 namespace clv {
 
-// Decode parameters after validation. Strides are in elements.
+// What turns a pair of attention rows into a row of differential attention:
+//   o = a_1 - lambda a_2,  out = o * out_scale * (weight / sqrt(mean(o^2) + eps), if any).
+struct DiffParams {
+  const float *lam;          // lambda[row * lam_row + head * lam_head]; null: lam_value
+  int64_t lam_row, lam_head;
+  float lam_value;
+  const float *weight;       // [head_dim] of the norm over a head's row; null: no norm
+  float eps, out_scale;
+};
+
+// Decode parameters after validation. Strides are in elements. Differential
+// decode counts rows of both maps: num_heads and group are twice the number of
+// query heads (row r of a kv head is map r % 2 of its query head r / 2).
 struct DecodeParams {
   void *out;
   const void *q;
@@ -66,6 +78,7 @@ struct DecodeParams {
   int32_t kv_fp8;
   const float *k_scales;  // [num_kv_heads]
   const float *v_scales;  // [num_kv_heads]
+  DiffParams diff;        // differential decode only
 };
 
 // Largest segment count the balanced mode keeps in LDS.
@@ -102,6 +115,21 @@ struct PrefillParams {
   // Compute units per XCD (the device's count / 8), for the prefill's
   // dispatch order; 0 keeps the natural order.
   int32_t cus_per_xcd;
+  DiffParams diff;  // differential prefill only
+};
+
+// One step of the block tables (tables.hip) after validation.
+struct TablesParams {
+  int32_t *block_tables;  // [rows, width]
+  const int32_t *blocks_held, *context_lens, *new_lens;  // [rows]
+  int32_t *free_blocks;   // [num_blocks]
+  const int32_t *num_free;
+  int32_t *blocks_held_out, *context_lens_out, *num_free_out;  // may be the inputs
+  int64_t *slot_mapping;  // [num_tokens]
+  int32_t *query_start_loc;  // [rows + 1]
+  int32_t *status;
+  int64_t num_tokens;
+  int32_t rows, width, block_shift, num_blocks, reserve;
 };
 
 constexpr int kPrefillDescBytes = 32;
@@ -167,6 +195,17 @@ bool prefill_f32_chosen(const PrefillParams &p, int block_size);
 PrefillSplitShape prefill_f32_split_shape(const PrefillParams &p);
 hipError_t launch_prefill_f32(const PrefillParams &p, const PrefillSplit *sp, hipStream_t stream);
 hipError_t launch_prefill_valu(const PrefillParams &p, DType dt, hipStream_t stream);
+// Differential attention (DecodeParams::diff / PrefillParams::diff): the forms
+// of the launchers above over rows of both maps, their epilogues and merges
+// joining each pair of rows.
+hipError_t launch_diff_decode_mfma(const DecodeParams &p, DType dt, hipStream_t stream);
+hipError_t launch_diff_decode_valu(const DecodeParams &p, DType dt, hipStream_t stream);
+hipError_t launch_diff_decode_stream(const DecodeParams &p, DType dt, hipStream_t stream);
+hipError_t launch_diff_stream_reduce(const DecodeParams &p, DType dt, hipStream_t stream);
+// A step of the block tables; workspace: tables_workspace_bytes (0: none).
+size_t tables_workspace_bytes(const TablesParams &p);
+hipError_t launch_tables(const TablesParams &p, void *workspace, hipStream_t stream);
+hipError_t launch_diff_prefill_valu(const PrefillParams &p, DType dt, hipStream_t stream);
 
 // Whether the MFMA decode kernel covers this shape/dtype.
 bool decode_mfma_supported(DType dt, int head_dim, int block_size);
@@ -175,5 +214,7 @@ bool decode_stream_supported(DType dt, int head_dim, int block_size, int64_t num
 // for this shape; otherwise launch_append_by_table runs first.
 bool stream_appends_in_kernel(DType dt, int head_dim, int block_size, int group);
 bool prefill_mfma_supported(DType dt, int head_dim, int block_size);
+// Whether the MFMA waves cover this differential decode.
+bool diff_decode_mfma_supported(int head_dim, int block_size);
 
 }  // namespace clv

@@ -57,6 +57,12 @@ __device__ __forceinline__ OutDesc<T> out_desc(const DecodeParams &p, int s, int
   return od;
 }
 
+// Differential decode: the output row of row r0 (even) of sequence s.
+template <typename T>
+__device__ __forceinline__ T *diff_out(const DecodeParams &p, int s, int r0) {
+  return (T *)p.out + (int64_t)s * p.out_stride_seq + (int64_t)(r0 / 2) * p.out_stride_head;
+}
+
 // ---------------------------------------------------------------- MFMA kernel
 // One workgroup (NW waves) per (sequence, kv head, 16-row query chunk,
 // partition); wave w takes the partition's 16-token steps w, w + NW, ...
@@ -75,11 +81,15 @@ __device__ __forceinline__ OutDesc<T> out_desc(const DecodeParams &p, int s, int
 // taking kv head HG * (blockIdx.y / n_gchunks) + w over the same partition,
 // so that the rows of a token for HG adjacent kv heads are read together (one
 // contiguous range of the token's row in the pools).
-template <typename T, int D, int NW, bool UNI, bool APPEND = false, int HG = 1>
+//
+// DIFF (single pass): differential attention, the rows of both maps (DiffRows),
+// joined where the waves' partials are merged.
+template <typename T, int D, int NW, bool UNI, bool APPEND = false, int HG = 1, bool DIFF = false>
 __global__ void __launch_bounds__(NW * HG * 64)
 paged_decode_mfma(const DecodeParams p, const int32_t *__restrict__ tables) {
   static_assert(HG == 1 || (NW == 1 && !APPEND), "head groups: one wave per kv head");
-  typedef typename GridWave<T, D, UNI>::type W;
+  static_assert(!DIFF || (HG == 1 && !APPEND), "differential decode: one pass over the pools");
+  typedef typename WaveRows<typename GridWave<T, D, UNI>::type, DIFF>::type W;
   __shared__ WaveSmem<NW, 16, D> sms[HG];
 
   const int hw = HG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
@@ -188,12 +198,16 @@ paged_decode_mfma(const DecodeParams p, const int32_t *__restrict__ tables) {
     }
   }
   __syncthreads();
-  merge_and_store<T, NW, 16, D>(sm, ng, out_desc<T>(p, s, h0, blockIdx.x),
-                                HG > 1 ? (int)(threadIdx.x & 63) : (int)threadIdx.x);
+  if constexpr (DIFF)
+    diff_merge_and_store<T, NW, 16, D>(sm, ng, p.diff, s, h0 / 2, diff_out<T>(p, s, h0),
+                                       p.out_stride_head);
+  else
+    merge_and_store<T, NW, 16, D>(sm, ng, out_desc<T>(p, s, h0, blockIdx.x),
+                                  HG > 1 ? (int)(threadIdx.x & 63) : (int)threadIdx.x);
 }
 
 // ---------------------------------------------------------------- VALU kernel
-template <typename T, int D, int GM, int NW>
+template <typename T, int D, int GM, int NW, bool DIFF = false>
 __global__ void __launch_bounds__(NW * 64) paged_decode_valu(const DecodeParams p) {
   __shared__ WaveSmem<NW, GM, D> sm;
   const int s = blockIdx.z;
@@ -209,11 +223,16 @@ __global__ void __launch_bounds__(NW * 64) paged_decode_valu(const DecodeParams 
     if (t_begin >= ctx) return;
     t_end = min(ctx, t_begin + p.partition_size);
   }
-  const T *q0 = (const T *)p.q + (int64_t)s * p.q_stride_seq + (int64_t)h0 * p.q_stride_head;
-  valu_attend<T, D, GM, NW>(q0, p.q_stride_head, ng, kv_view<T>(p, s, kvh), t_begin, t_end,
-                            p.scale_log2, sm);
+  const T *q0 = (const T *)p.q + (int64_t)s * p.q_stride_seq +
+                (int64_t)(DIFF ? h0 / 2 : h0) * p.q_stride_head;
+  valu_attend<T, D, GM, NW, DIFF>(q0, p.q_stride_head, ng, kv_view<T>(p, s, kvh), t_begin, t_end,
+                                  p.scale_log2, sm);
   __syncthreads();
-  merge_and_store<T, NW, GM, D>(sm, ng, out_desc<T>(p, s, h0, blockIdx.x));
+  if constexpr (DIFF)
+    diff_merge_and_store<T, NW, GM, D>(sm, ng, p.diff, s, h0 / 2, diff_out<T>(p, s, h0),
+                                       p.out_stride_head);
+  else
+    merge_and_store<T, NW, GM, D>(sm, ng, out_desc<T>(p, s, h0, blockIdx.x));
 }
 
 // ---------------------------------------------------------------- split-K reduce
@@ -322,6 +341,53 @@ hipError_t launch_valu_t(const DecodeParams &p, hipStream_t stream) {
   }
 }
 
+// Differential decode, one workgroup per (sequence, kv head, 16-row chunk).
+template <typename T, int D>
+hipError_t launch_diff_mfma_td(const DecodeParams &p, hipStream_t stream) {
+  const dim3 grid(1u, (unsigned)(p.num_kv_heads * p.n_gchunks), (unsigned)p.num_seqs);
+  if (p.block_shift >= 4)
+    hipLaunchKernelGGL((paged_decode_mfma<T, D, 4, true, false, 1, true>), grid, dim3(256), 0,
+                       stream, p, p.block_tables);
+  else
+    hipLaunchKernelGGL((paged_decode_mfma<T, D, 4, false, false, 1, true>), grid, dim3(256), 0,
+                       stream, p, p.block_tables);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_diff_mfma_t(const DecodeParams &p, hipStream_t stream) {
+  switch (p.head_dim) {
+    case 64: return launch_diff_mfma_td<T, 64>(p, stream);
+    case 128: return launch_diff_mfma_td<T, 128>(p, stream);
+    case 256: return launch_diff_mfma_td<T, 256>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+template <typename T, int D>
+hipError_t launch_diff_valu_td(const DecodeParams &p, hipStream_t stream) {
+  constexpr int NW = D >= 256 ? 2 : 4;
+  const dim3 grid(1u, (unsigned)(p.num_kv_heads * p.n_gchunks), (unsigned)p.num_seqs);
+  if (p.group <= 4)
+    hipLaunchKernelGGL((paged_decode_valu<T, D, 4, NW, true>), grid, dim3(NW * 64), 0, stream, p);
+  else
+    hipLaunchKernelGGL((paged_decode_valu<T, D, 16, NW, true>), grid, dim3(NW * 64), 0, stream, p);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_diff_valu_t(const DecodeParams &p, hipStream_t stream) {
+  switch (p.head_dim) {
+    case 8: return launch_diff_valu_td<T, 8>(p, stream);
+    case 16: return launch_diff_valu_td<T, 16>(p, stream);
+    case 32: return launch_diff_valu_td<T, 32>(p, stream);
+    case 64: return launch_diff_valu_td<T, 64>(p, stream);
+    case 128: return launch_diff_valu_td<T, 128>(p, stream);
+    case 256: return launch_diff_valu_td<T, 256>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
 template <typename T>
 hipError_t launch_reduce_t(const DecodeParams &p, hipStream_t stream) {
   const int64_t rows = (int64_t)p.num_seqs * p.num_heads;
@@ -369,6 +435,26 @@ hipError_t launch_decode_valu(const DecodeParams &p, DType dt, hipStream_t strea
     case DType::F16: return launch_valu_t<_Float16>(p, stream);
     case DType::BF16: return launch_valu_t<__bf16>(p, stream);
   }
+  return hipErrorInvalidValue;
+}
+
+bool diff_decode_mfma_supported(int head_dim, int block_size) {
+  return (head_dim == 64 || head_dim == 128 || head_dim == 256) && block_size >= 4;
+}
+
+hipError_t launch_diff_decode_mfma(const DecodeParams &p, DType dt, hipStream_t stream) {
+  if (p.partition_size != 0 || p.kv_fp8) return hipErrorInvalidValue;
+  if (dt == DType::BF16) return launch_diff_mfma_t<__bf16>(p, stream);
+  if (dt == DType::F16) return launch_diff_mfma_t<_Float16>(p, stream);
+  if (dt == DType::F32) return launch_diff_mfma_t<float>(p, stream);
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_diff_decode_valu(const DecodeParams &p, DType dt, hipStream_t stream) {
+  if (p.partition_size != 0 || p.kv_fp8) return hipErrorInvalidValue;
+  if (dt == DType::BF16) return launch_diff_valu_t<__bf16>(p, stream);
+  if (dt == DType::F16) return launch_diff_valu_t<_Float16>(p, stream);
+  if (dt == DType::F32) return launch_diff_valu_t<float>(p, stream);
   return hipErrorInvalidValue;
 }
 

@@ -22,9 +22,12 @@
 
 namespace clv {
 
+typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+
 template <int CH> struct VChunk;
-template <> struct VChunk<8> { typedef u32x4 type; };  // D = 128: 16 bytes per lane
-template <> struct VChunk<4> { typedef u32x2 type; };  // D = 64: 8 bytes per lane
+template <> struct VChunk<16> { typedef u32x8 type; };  // D = 256: two 16-byte words per lane
+template <> struct VChunk<8> { typedef u32x4 type; };   // D = 128: 16 bytes per lane
+template <> struct VChunk<4> { typedef u32x2 type; };   // D = 64: 8 bytes per lane
 
 // Clamp a context length to what the grid and the block table cover.
 __device__ __forceinline__ int clamp_ctx(const DecodeParams &p, int s) {
@@ -91,7 +94,10 @@ __device__ __forceinline__ u32x4 fp8x8_to(u32x2 w) {
 // UNI: block_size >= 16, so a step sits in one block and its block-table
 // entry is wave-uniform (scalar load, buffer loads). Otherwise (block_size 4
 // or 8) lanes look up their own rows.
-// KT (UNI, head_dim 128): K is loaded like V, whole 256-byte rows with the
+// D = 256: a lane's chunk of a row is two words, 128 columns apart (each load
+// instruction still reads 256 consecutive bytes of four rows), so accumulator
+// element m of lane group n16 is column 128 (m / 8) + 8 n16 + m % 8.
+// KT (UNI, head_dim 128 or 256): K is loaded like V, whole 256-byte rows with the
 // streaming policy (four rows per instruction), and turned into the MFMA A
 // layout through a per-wave LDS buffer of 16 rows (set_k_lds). A pure read of
 // that pattern runs about 3 % faster than the A-layout loads, which read half
@@ -109,22 +115,26 @@ struct DecodeWave {
   typedef typename MfV::op_t pv_t;
   static constexpr int NQK = D / 32;  // QK MFMAs per step
   static constexpr int CH = D / 16;   // V elements per lane per token = PV output blocks
+  static constexpr int WORDS = CH > 8 ? CH / 8 : 1;  // words of a lane's chunk of a row
+  static constexpr int WC = CH / WORDS;              // columns of a word
   static constexpr int EB = (int)sizeof(T);
   static constexpr int STEP = 16;
   // LDS row stride of the K transpose buffer: 32 mod 64 bytes keeps both the
   // row writes and the A-layout reads (lane row = lane % 16) conflict-free.
   static constexpr int KT_ROW = D * EB + 32;
   static constexpr int KT_BYTES = KT ? 16 * KT_ROW : 16;  // 16: no transpose buffer
-  static_assert(!KT || (UNI && D == 128), "K transpose needs block_size >= 16 and head_dim 128");
+  static_assert(!KT || (UNI && D >= 128), "K transpose needs block_size >= 16 and whole 256-byte rows");
   static_assert(!KV8 || KT, "fp8 pools are read on the K-transpose path");
   static constexpr int EBC = KV8 ? 1 : EB;  // bytes per cache element
   typedef typename VChunk<CH>::type vchunk_t;
+  typedef uint32_t v8_t __attribute__((ext_vector_type(2 * WORDS)));  // KV8: fp8 chunk of a row
 
   // Loads of one step: K rows (lane row n16) and the V rows 4j..4j+3.
   struct Regs {
     u32x4 k[NQK];
     vchunk_t v[4];
-    u32x2 k8[KV8 ? NQK : 1], v8[KV8 ? 4 : 1];  // KV8: the loaded fp8 values
+    u32x2 k8[KV8 ? NQK : 1];  // KV8: the loaded fp8 values
+    v8_t v8[KV8 ? 4 : 1];
     bool ok;  // the lane's V rows lie in a readable block
   };
 
@@ -153,7 +163,7 @@ struct DecodeWave {
     scale_log2 = p.scale_log2;
     k_lane = (uint32_t)(n16 * stok + 8 * j * EB);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v_lane[r] = (uint32_t)((4 * j + r) * stok + n16 * CH * EBC);
+    for (int r = 0; r < 4; ++r) v_lane[r] = (uint32_t)((4 * j + r) * stok + n16 * WC * EBC);
     vscale = 1.f;
     reset();
   }
@@ -161,7 +171,20 @@ struct DecodeWave {
   // Output column of accumulator element m in lane group n16 (o[m] holds
   // O[g = 4j + r][col_of(n16, m)]; four consecutive m from a multiple of 4
   // are four consecutive columns).
-  __device__ __forceinline__ static int col_of(int n16, int m) { return n16 * CH + m; }
+  __device__ __forceinline__ static int col_of(int n16, int m) {
+    return (m / WC) * (D / WORDS) + n16 * WC + m % WC;
+  }
+
+  // A lane's chunk of a V row: `load(byte offset past its first word)` per word.
+  template <typename F>
+  __device__ __forceinline__ static vchunk_t load_chunk(F load) {
+    if constexpr (WORDS == 1) {
+      return load(0u);
+    } else {
+      const u32x4 a = load(0u), b = load((uint32_t)(D / WORDS * EB));
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
 
   // KV8: the scales of the kv head a run reads (the key scale times the
   // softmax scale in the log2 domain, and the value scale).
@@ -215,19 +238,33 @@ struct DecodeWave {
     const rsrc_t rv = make_rsrc(vbase + off);
     if constexpr (KV8) {
 #pragma unroll
-      for (int i = 0; i < NQK; ++i) R.k8[i] = buf_load<u32x2, kCacheStream>(rk, v_lane[i]);
+      for (int i = 0; i < NQK; ++i)
+        R.k8[i] = buf_load<u32x2, kCacheStream>(rk, v_lane[i & 3] + (i >> 2) * (D / WORDS));
 #pragma unroll
-      for (int r = 0; r < 4; ++r) R.v8[r] = buf_load<u32x2, kCacheStream>(rv, v_lane[r]);
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (WORDS == 1) {
+          R.v8[r] = buf_load<u32x2, kCacheStream>(rv, v_lane[r]);
+        } else {
+          const u32x2 a = buf_load<u32x2, kCacheStream>(rv, v_lane[r]);
+          const u32x2 b = buf_load<u32x2, kCacheStream>(rv, v_lane[r] + D / WORDS);
+          R.v8[r] = __builtin_shufflevector(a, b, 0, 1, 2, 3);
+        }
+      }
       return;
     } else if constexpr (KT) {
 #pragma unroll
-      for (int i = 0; i < NQK; ++i) R.k[i] = buf_load<u32x4, kCacheStream>(rk, v_lane[i]);
+      for (int i = 0; i < NQK; ++i)
+        R.k[i] = buf_load<u32x4, kCacheStream>(rk, v_lane[i & 3] + (i >> 2) * (D / WORDS * EB));
     } else {
 #pragma unroll
       for (int i = 0; i < NQK; ++i) R.k[i] = buf_load<u32x4, kCacheDefault>(rk, k_lane + 64u * i);
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) R.v[r] = buf_load<vchunk_t, kCacheStream>(rv, v_lane[r]);
+    for (int r = 0; r < 4; ++r)
+      R.v[r] = load_chunk([&](uint32_t at) {
+        typedef typename VChunk<WC>::type word_t;
+        return buf_load<word_t, kCacheStream>(rv, v_lane[r] + at);
+      });
   }
 
   __device__ __forceinline__ void set_k_lds(char *buf) { k_lds = buf; }
@@ -239,7 +276,7 @@ struct DecodeWave {
     vchunk_t v;
   };
   __device__ __forceinline__ void load_new(const T *knew, const T *vnew, NewRow &nr) const {
-    static_assert(KT, "the fused append mirrors the K-transpose loads");
+    static_assert(KT && D == 128, "the fused append mirrors the K-transpose loads");
     nr.k = load_vec<u32x4>(knew + n16 * CH);
     nr.v = load_vec<vchunk_t>(vnew + n16 * CH);
   }
@@ -278,11 +315,15 @@ struct DecodeWave {
       const int vb = tv < g.t_end ? g.bt[tv >> bshift] : 0;
       const bool vok = tv < g.t_end && (unsigned)vb < nblocks;
       R.ok = vok;
-      const int64_t voff = (vok ? vb * sblk + (tv & bmask) * stok : 0) + n16 * CH * EB;
+      const int64_t voff = (vok ? vb * sblk + (tv & bmask) * stok : 0) + n16 * WC * EB;
 #pragma unroll
       for (int i = 0; i < NQK; ++i) R.k[i] = load_vec<u32x4>(g.kbase + koff + 64 * i);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) R.v[r] = load_vec<vchunk_t>(g.vbase + voff + r * stok);
+      for (int r = 0; r < 4; ++r)
+        R.v[r] = load_chunk([&](uint32_t at) {
+          typedef typename VChunk<WC>::type word_t;
+          return load_vec<word_t>(g.vbase + voff + r * stok + at);
+        });
     }
   }
 
@@ -296,12 +337,13 @@ struct DecodeWave {
       for (int i = 0; i < NQK; ++i) R.k[i] = fp8x8_to<T>(R.k8[i]);
     }
     if constexpr (KT) {
-      // R.k[i] holds row 4j + i, bytes 16 n16 .. +16 (the V pattern). Through
-      // LDS into the A layout: row n16, bytes 64 i + 16 j .. +16. A wave's LDS
-      // operations run in order, so the reads see this step's writes and the
-      // next step's writes come after these reads.
+      // R.k[i] holds row 4j + i % 4, bytes 256 (i / 4) + 16 n16 .. +16 (the V
+      // pattern). Through LDS into the A layout: row n16, bytes 64 i + 16 j .. +16.
+      // A wave's LDS operations run in order, so the reads see this step's writes
+      // and the next step's writes come after these reads.
 #pragma unroll
-      for (int i = 0; i < NQK; ++i) store_vec<u32x4>(k_lds + (4 * j + i) * KT_ROW + 16 * n16, R.k[i]);
+      for (int i = 0; i < NQK; ++i)
+        store_vec<u32x4>(k_lds + (4 * j + (i & 3)) * KT_ROW + 256 * (i >> 2) + 16 * n16, R.k[i]);
 #pragma unroll
       for (int i = 0; i < NQK; ++i) R.k[i] = load_vec<u32x4>(k_lds + n16 * KT_ROW + 64 * i + 16 * j);
     }
@@ -321,7 +363,7 @@ struct DecodeWave {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if (x[r] == kNegInf) {  // keep NaN/Inf of unused slots out of P.V
-          if constexpr (KV8) R.v8[r] = (u32x2){0u, 0u};
+          if constexpr (KV8) R.v8[r] = v8_t{};
           else R.v[r] = z;
         }
       }
@@ -413,11 +455,11 @@ struct DecodeWave {
       if (g >= ng) continue;
       const int64_t row = row0 + g * rstride;
       const float inv = (l > 0.f ? 1.f / l : 0.f) * (KV8 ? vscale : 1.f);
-      float *dst = ws_o + row * D + n16 * CH;
+      float *dst = ws_o + row * D;
 #pragma unroll
       for (int m = 0; m < CH; m += 4) {
         const f32x4 v = {o[m][r] * inv, o[m + 1][r] * inv, o[m + 2][r] * inv, o[m + 3][r] * inv};
-        store_vec<f32x4>(dst + m, v);
+        store_vec<f32x4>(dst + col_of(n16, m), v);
       }
       if (n16 == 0) {
         ws_m[row] = l > 0.f ? mrow * kLn2 : kNegInf;
@@ -652,6 +694,44 @@ struct DecodeWaveF32 {
   }
 };
 
+// Differential rows: row r of a kv head is map r % 2 of its query head r / 2.
+// q holds both maps' halves (q1 | q2), a key row likewise (k1 | k2), so the
+// row is that half of q with zeros in the other one: its score over the whole
+// key row is q_m . k_m, both maps share the loaded K and V, and a wave runs the
+// step of plain attention over 2 x group rows. (The score MFMAs multiply as
+// many zeros; a step has 16 columns either way, and decode is bound by bytes.)
+template <class WV>
+struct DiffRows : WV {
+  typedef typename WV::qk_t qk_t;
+  static constexpr int NQK = WV::NQK;
+
+  __device__ __forceinline__ void load_q_raw(const DecodeParams &p, int s, int r0, int nr,
+                                             u32x4 (&raw)[NQK]) const {
+    // r0 is even (kv head * 2 group + a multiple of 16).
+    const int row = min(this->n16, nr - 1);
+    const char *q = (const char *)p.q + ((int64_t)s * p.q_stride_seq +
+                                         (int64_t)((r0 + row) >> 1) * p.q_stride_head) * WV::EB;
+#pragma unroll
+    for (int i = 0; i < NQK; ++i) raw[i] = load_vec<u32x4>(q + 64 * i + 16 * this->j);
+  }
+  __device__ __forceinline__ void mask_q(const u32x4 (&raw)[NQK], int nr, qk_t (&q)[NQK]) const {
+#pragma unroll
+    for (int i = 0; i < NQK; ++i) {
+      const bool keep = this->n16 < nr && (i >= NQK / 2) == ((this->n16 & 1) != 0);
+      q[i] = __builtin_bit_cast(qk_t, keep ? raw[i] : (u32x4){0u, 0u, 0u, 0u});
+    }
+  }
+  __device__ __forceinline__ void load_q(const DecodeParams &p, int s, int r0, int nr,
+                                         qk_t (&q)[NQK]) const {
+    u32x4 raw[NQK];
+    load_q_raw(p, s, r0, nr, raw);
+    mask_q(raw, nr, q);
+  }
+};
+
+template <class WV, bool DIFF> struct WaveRows { typedef WV type; };
+template <class WV> struct WaveRows<WV, true> { typedef DiffRows<WV> type; };
+
 // The per-wave decode type of the grid kernel (paged_decode_mfma). K stays
 // in the A layout here: the K transpose of the stream kernel measured 6 %
 // slower in this kernel (16 x 32K-token split-K decode: 364 -> 387 us, also
@@ -668,7 +748,7 @@ struct GridWave<float, D, UNI> {
 // The per-wave decode type of the balanced stream kernel.
 template <typename T, int D, bool UNI, bool KV8>
 struct StreamWave {
-  typedef DecodeWave<T, D, UNI, UNI && D == 128, KV8> type;
+  typedef DecodeWave<T, D, UNI, UNI && D >= 128, KV8> type;
 };
 template <int D, bool UNI>
 struct StreamWave<float, D, UNI, false> {
@@ -691,15 +771,16 @@ struct StreamWave<float, D, UNI, false> {
 // a decode over a context can take one more token after its partials are
 // written. The score is xm = (sum over the wave of xdot) * xscale, summed
 // here after the rows' loads are issued so that its shuffles overlap them.
-template <typename T, int D, int NW, bool X = false>
-__device__ __forceinline__ void lse_merge(const float *m, const float *l, const float *c,
-                                          int64_t ms, int64_t cs, int n, T *dst, float *smem,
-                                          float xdot = 0.f, float xscale = 0.f,
-                                          const float *xv = nullptr) {
+// The merged row's element lane + 64 e comes back in res[e], in wave wv = 0 of
+// the NW (true; the others hold no result).
+template <int D, int NW, bool X = false>
+__device__ __forceinline__ bool lse_merge_row(const float *m, const float *l, const float *c,
+                                              int64_t ms, int64_t cs, int n, int wv, float *smem,
+                                              float (&res)[(D + 63) / 64], float xdot = 0.f,
+                                              float xscale = 0.f, const float *xv = nullptr) {
   constexpr int EPL = (D + 63) / 64;
   constexpr int R = NW > 1 ? 16 : 8;
   const int lane = threadIdx.x & 63;
-  const int wv = NW > 1 ? (int)(threadIdx.x >> 6) : 0;
   const int C = NW > 1 ? max(1, min(64, (n + NW - 1) / NW)) : 64;
   // The row's max needs every m_i; the first chunk's (m, l) and its first
   // R context rows are loaded together, before any reduction, so that a
@@ -771,7 +852,7 @@ __device__ __forceinline__ void lse_merge(const float *m, const float *l, const 
     for (int e = 0; e < EPL; ++e)
       if (lane + 64 * e < D) sa[wv * D + lane + 64 * e] = acc[e];
     __syncthreads();
-    if (wv != 0) return;
+    if (wv != 0) return false;
     L = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) L += sl[w];
@@ -791,8 +872,25 @@ __device__ __forceinline__ void lse_merge(const float *m, const float *l, const 
   }
   const float inv = 1.f / fmaxf(L, 1e-12f);
 #pragma unroll
+  for (int e = 0; e < EPL; ++e) res[e] = acc[e] * inv;
+  return true;
+}
+
+// lse_merge_row with the row written to dst.
+template <typename T, int D, int NW, bool X = false>
+__device__ __forceinline__ void lse_merge(const float *m, const float *l, const float *c,
+                                          int64_t ms, int64_t cs, int n, T *dst, float *smem,
+                                          float xdot = 0.f, float xscale = 0.f,
+                                          const float *xv = nullptr) {
+  constexpr int EPL = (D + 63) / 64;
+  const int lane = threadIdx.x & 63;
+  float res[EPL];
+  if (!lse_merge_row<D, NW, X>(m, l, c, ms, cs, n, NW > 1 ? (int)(threadIdx.x >> 6) : 0, smem, res,
+                               xdot, xscale, xv))
+    return;
+#pragma unroll
   for (int e = 0; e < EPL; ++e)
-    if (lane + 64 * e < D) dst[lane + 64 * e] = from_f32<T>(acc[e] * inv);
+    if (lane + 64 * e < D) dst[lane + 64 * e] = from_f32<T>(res[e]);
 }
 
 }  // namespace clv

@@ -169,8 +169,10 @@ struct AppendRow<WV, true> {
 // partitions through one ring and writes each partition's partial, in the
 // split-K layout [sequence, query head, partition] that splitk_reduce
 // merges, when the partition's last step is folded.
+// DIFF: differential attention, the rows of both maps (DiffRows); the merge
+// joins them.
 template <typename T, int D, bool UNI, int DEPTH, bool APPEND = false, bool KV8 = false,
-          bool PART = false>
+          bool PART = false, bool DIFF = false>
 __global__ void __launch_bounds__(kThreads)
 paged_decode_stream(const DecodeParams p, const int32_t *__restrict__ tables,
                     const int32_t *__restrict__ lens, float *__restrict__ ws_o,
@@ -179,7 +181,7 @@ paged_decode_stream(const DecodeParams p, const int32_t *__restrict__ tables,
   // Every global pointer is a separate restrict argument: with stores to the
   // workspace inside the main loop, that is what lets the compiler keep the
   // wave-uniform block-table reads scalar loads.
-  typedef typename StreamWave<T, D, UNI, KV8>::type WV;
+  typedef typename WaveRows<typename StreamWave<T, D, UNI, KV8>::type, DIFF>::type WV;
   constexpr int CEB = KV8 ? 1 : (int)sizeof(T);
   typedef typename WV::qk_t qk_t;
   __shared__ __attribute__((aligned(16))) char s_kt[kWaves][WV::KT_BYTES];
@@ -418,6 +420,42 @@ paged_decode_stream(const DecodeParams p, const int32_t *__restrict__ tables,
   }
 }
 
+// The partials of one row (query row `gall` of kv head kvh of sequence s) that
+// the stream kernel left: their count n, and the workspace row of the first
+// (the others follow at a stride of 16 * head_group rows).
+__device__ __forceinline__ int64_t row_partials(const DecodeParams &p, int s, int kvh, int gall,
+                                                int &n) {
+  const int HG = p.head_group;
+  const int kvg = kvh / HG, wk = kvh - kvg * HG;
+  const int seg = (s * (p.num_kv_heads / HG) + kvg) * p.n_gchunks + gall / 16;
+  const int g = gall % 16;
+  // The segment bounds and the step total are wave-uniform and read-only
+  // here: three scalar loads issued together, one wait (the split's
+  // arithmetic then runs on the scalar unit).
+  int a, b, n_total;
+  {
+    const int32_t *ps = p.seg_prefix + __builtin_amdgcn_readfirstlane(seg);
+    const int32_t *pn = p.seg_prefix + p.num_segments;
+    uint64_t ab;
+    // Early-clobber outputs: the first load's destination is written when its
+    // data returns, so it must not share registers with the second's address.
+    asm volatile("s_load_dwordx2 %0, %2, 0x0\n\ts_load_dword %1, %3, 0x0\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&s"(ab), "=&s"(n_total) : "s"(ps), "s"(pn) : "memory");
+    a = (int)(uint32_t)ab + p.stream_run_cost;
+    b = (int)(uint32_t)(ab >> 32);
+  }
+  const int64_t N = n_total;
+  const int64_t W = min((int64_t)(p.num_waves / HG), N);
+  int w0 = 0;
+  n = 0;
+  if (b > a) {
+    const StreamSplit split(p, W, N);
+    w0 = split.owner(a);
+    n = split.owner(b - 1) - w0 + 1;
+  }
+  return (n > 0 ? (((int64_t)seg + w0) * HG + wk) * 16 : 0) + g;
+}
+
 // NW waves per (sequence, query head): one, four rows to a workgroup, or
 // kMergeWaves, one row to a workgroup (launch_sreduce_t chooses).
 // NEW: the partials cover context_lens[s] tokens and the merge takes
@@ -460,33 +498,8 @@ __global__ void __launch_bounds__(NW > 1 ? NW * 64 : 256) stream_reduce(const De
     if (gall == 0) slot = p.slot_mapping[s];
   }
   const int HG = p.head_group;
-  const int kvg = kvh / HG, wk = kvh - kvg * HG;
-  const int seg = (s * (p.num_kv_heads / HG) + kvg) * p.n_gchunks + gall / 16;
-  const int g = gall % 16;
-  // The segment bounds and the step total are wave-uniform and read-only
-  // here: three scalar loads issued together, one wait (the split's
-  // arithmetic then runs on the scalar unit).
-  int a, b, n_total;
-  {
-    const int32_t *ps = p.seg_prefix + __builtin_amdgcn_readfirstlane(seg);
-    const int32_t *pn = p.seg_prefix + p.num_segments;
-    uint64_t ab;
-    // Early-clobber outputs: the first load's destination is written when its
-    // data returns, so it must not share registers with the second's address.
-    asm volatile("s_load_dwordx2 %0, %2, 0x0\n\ts_load_dword %1, %3, 0x0\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&s"(ab), "=&s"(n_total) : "s"(ps), "s"(pn) : "memory");
-    a = (int)(uint32_t)ab + p.stream_run_cost;
-    b = (int)(uint32_t)(ab >> 32);
-  }
-  const int64_t N = n_total;
-  const int64_t W = min((int64_t)(p.num_waves / HG), N);
-  int n = 0, w0 = 0;
-  if (b > a) {
-    const StreamSplit split(p, W, N);
-    w0 = split.owner(a);
-    n = split.owner(b - 1) - w0 + 1;
-  }
-  const int64_t row0 = (n > 0 ? (((int64_t)seg + w0) * HG + wk) * 16 : 0) + g;
+  int n;
+  const int64_t row0 = row_partials(p, s, kvh, gall, n);
   T *dst = (T *)p.out + (int64_t)s * p.out_stride_seq + (int64_t)h * p.out_stride_head;
   if constexpr (!NEW) {
     lse_merge<T, D, NW>(p.ws_m + row0, p.ws_l + row0, p.ws_o + row0 * D, 16 * HG, 16 * HG * D, n,
@@ -523,6 +536,57 @@ __global__ void __launch_bounds__(NW > 1 ? NW * 64 : 256) stream_reduce(const De
         }
       }
     }
+  }
+}
+
+// Merge of a differential decode: NW waves per row of a map, so 2 NW per
+// (sequence, query head); the first map's wave joins the pair, normalises and
+// writes it. A workgroup holds two pairs at NW = 1, one otherwise.
+template <typename T, int D, int NW>
+__global__ void __launch_bounds__(NW > 1 ? 2 * NW * 64 : 256)
+diff_stream_reduce(const DecodeParams p) {
+  constexpr int EPL = (D + 63) / 64;
+  constexpr int PAIRS = NW > 1 ? 1 : 2;
+  __shared__ float smem[NW > 1 ? 2 : 1][NW > 1 ? NW * (D + 1) : 1];
+  __shared__ float s_second[PAIRS][D];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int slot = NW > 1 ? 0 : wave >> 1;
+  const int map = NW > 1 ? wave / NW : wave & 1;
+  const int heads = p.num_heads / 2;
+  const int64_t idx = (int64_t)blockIdx.x * PAIRS + slot;
+  const bool any = idx < (int64_t)p.num_seqs * heads;
+  const int s = any ? (int)(idx / heads) : 0;
+  const int h = any ? (int)(idx - (int64_t)s * heads) : 0;
+  const int kvh = h / (p.group / 2);
+  int n;
+  const int64_t row0 = row_partials(p, s, kvh, 2 * h - kvh * p.group + map, n);
+  const int HG = p.head_group;
+  float a[EPL];
+  const bool mine = lse_merge_row<D, NW>(p.ws_m + row0, p.ws_l + row0, p.ws_o + row0 * D, 16 * HG,
+                                         16 * HG * D, n, NW > 1 ? wave % NW : 0,
+                                         smem[NW > 1 ? map : 0], a);
+  if (mine && map == 1)
+#pragma unroll
+    for (int e = 0; e < EPL; ++e)
+      if (lane + 64 * e < D) s_second[slot][lane + 64 * e] = a[e];
+  __syncthreads();
+  if (!mine || map == 1 || !any) return;
+  const float lam = diff_lambda(p.diff, s, h);
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) {
+    a[e] = lane + 64 * e < D ? a[e] - lam * s_second[slot][lane + 64 * e] : 0.f;
+    ss += a[e] * a[e];
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) ss += shfl_xor(ss, off);
+  const float f = diff_factor(p.diff, ss, D);
+  T *dst = (T *)p.out + (int64_t)s * p.out_stride_seq + (int64_t)h * p.out_stride_head;
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) {
+    const int d = lane + 64 * e;
+    if (d < D) dst[d] = from_f32<T>(a[e] * (p.diff.weight != nullptr ? f * p.diff.weight[d] : f));
   }
 }
 
@@ -615,7 +679,80 @@ hipError_t launch_sreduce_t(const DecodeParams &p, hipStream_t stream) {
   return launch_sreduce_tn<T, NEW, 1>(p, stream);
 }
 
+// Ring depth of the differential decode: as for plain decode at the same bytes
+// per step (16-bit pools three steps of up to 8 KiB a wave, two of 16 KiB).
+template <typename T, int D, bool KV8>
+hipError_t launch_diff_stream_td(const DecodeParams &p, hipStream_t stream) {
+  constexpr int DEPTH = D * (KV8 ? 1 : (int)sizeof(T)) > 256 ? 2 : 3;
+  const dim3 grid((unsigned)((p.num_waves + kWaves - 1) / kWaves));
+  if (p.block_shift >= 4)
+    hipLaunchKernelGGL((paged_decode_stream<T, D, true, DEPTH, false, KV8, false, true>), grid,
+                       dim3(kThreads), 0, stream, p, p.block_tables, p.context_lens, p.ws_o,
+                       p.ws_m, p.ws_l, p.seg_prefix);
+  else if constexpr (!KV8)
+    hipLaunchKernelGGL((paged_decode_stream<T, D, false, DEPTH, false, false, false, true>), grid,
+                       dim3(kThreads), 0, stream, p, p.block_tables, p.context_lens, p.ws_o,
+                       p.ws_m, p.ws_l, p.seg_prefix);
+  else
+    return hipErrorInvalidValue;
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_diff_stream_t(const DecodeParams &p, hipStream_t stream) {
+  if constexpr (sizeof(T) == 2) {
+    if (p.kv_fp8)
+      return p.head_dim == 128 ? launch_diff_stream_td<T, 128, true>(p, stream)
+                               : hipErrorInvalidValue;
+  }
+  if (p.kv_fp8) return hipErrorInvalidValue;
+  switch (p.head_dim) {
+    case 64: return launch_diff_stream_td<T, 64, false>(p, stream);
+    case 128: return launch_diff_stream_td<T, 128, false>(p, stream);
+    case 256: return launch_diff_stream_td<T, 256, false>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+template <typename T, int D>
+hipError_t launch_diff_sreduce_td(const DecodeParams &p, hipStream_t stream) {
+  const int64_t pairs = (int64_t)p.num_seqs * (p.num_heads / 2);
+  const int64_t groups = p.num_waves / p.head_group;
+  if (groups > (int64_t)kWideMergePartials * p.num_segments)
+    hipLaunchKernelGGL((diff_stream_reduce<T, D, kMergeWaves>), dim3((unsigned)pairs),
+                       dim3(2 * kMergeWaves * 64), 0, stream, p);
+  else
+    hipLaunchKernelGGL((diff_stream_reduce<T, D, 1>), dim3((unsigned)((pairs + 1) / 2)), dim3(256),
+                       0, stream, p);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_diff_sreduce_t(const DecodeParams &p, hipStream_t stream) {
+  switch (p.head_dim) {
+    case 64: return launch_diff_sreduce_td<T, 64>(p, stream);
+    case 128: return launch_diff_sreduce_td<T, 128>(p, stream);
+    case 256: return launch_diff_sreduce_td<T, 256>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
 }  // namespace
+
+hipError_t launch_diff_decode_stream(const DecodeParams &p, DType dt, hipStream_t stream) {
+  if (p.append_new || p.partition_size != 0) return hipErrorInvalidValue;
+  if (dt == DType::BF16) return launch_diff_stream_t<__bf16>(p, stream);
+  if (dt == DType::F16) return launch_diff_stream_t<_Float16>(p, stream);
+  if (dt == DType::F32) return launch_diff_stream_t<float>(p, stream);
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_diff_stream_reduce(const DecodeParams &p, DType dt, hipStream_t stream) {
+  if (dt == DType::BF16) return launch_diff_sreduce_t<__bf16>(p, stream);
+  if (dt == DType::F16) return launch_diff_sreduce_t<_Float16>(p, stream);
+  if (dt == DType::F32) return launch_diff_sreduce_t<float>(p, stream);
+  return hipErrorInvalidValue;
+}
 
 bool decode_stream_supported(DType dt, int head_dim, int block_size, int64_t num_segments) {
   return decode_mfma_supported(dt, head_dim, block_size) && num_segments <= kStreamMaxSegments;

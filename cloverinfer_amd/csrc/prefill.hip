@@ -17,7 +17,9 @@
 namespace clv {
 namespace {
 
-template <typename T, int D, int GM, int NW>
+// DIFF: differential attention. p.group counts the rows of both maps (two per
+// query head of the kv head), which the epilogue joins.
+template <typename T, int D, int GM, int NW, bool DIFF = false>
 __global__ void __launch_bounds__(NW * 64) chunked_prefill_valu(const PrefillParams p) {
   __shared__ WaveSmem<NW, GM, D> sm;
   const int tok = blockIdx.x;
@@ -40,10 +42,10 @@ __global__ void __launch_bounds__(NW * 64) chunked_prefill_valu(const PrefillPar
   const int kvh = blockIdx.y / n_gchunks;
   const int g0 = (blockIdx.y - kvh * n_gchunks) * GM;
   const int ng = min(GM, p.group - g0);
-  const int h0 = kvh * p.group + g0;
+  const int h0 = DIFF ? (kvh * p.group + g0) / 2 : kvh * p.group + g0;  // first query head
   if (i >= p.max_query_len) {
     const T nan = (T)__builtin_nanf("");
-    for (int idx = threadIdx.x; idx < ng * D; idx += NW * 64)
+    for (int idx = threadIdx.x; idx < (DIFF ? ng / 2 : ng) * D; idx += NW * 64)
       ((T *)p.out)[(int64_t)tok * p.out_stride_token +
                    (int64_t)(h0 + idx / D) * p.out_stride_head + idx % D] = nan;
     return;
@@ -59,8 +61,14 @@ __global__ void __launch_bounds__(NW * 64) chunked_prefill_valu(const PrefillPar
   kv.num_blocks = (unsigned)p.num_blocks;
 
   const T *q0 = (const T *)p.q + (int64_t)tok * p.q_stride_token + (int64_t)h0 * p.q_stride_head;
-  valu_attend<T, D, GM, NW>(q0, p.q_stride_head, ng, kv, 0, limit, p.scale_log2, sm);
+  valu_attend<T, D, GM, NW, DIFF>(q0, p.q_stride_head, ng, kv, 0, limit, p.scale_log2, sm);
   __syncthreads();
+  if constexpr (DIFF) {
+    diff_merge_and_store<T, NW, GM, D>(sm, ng, p.diff, tok, h0,
+                                       (T *)p.out + (int64_t)tok * p.out_stride_token +
+                                           (int64_t)h0 * p.out_stride_head, p.out_stride_head);
+    return;
+  }
   OutDesc<T> od;
   od.split = false;
   od.out = (T *)p.out + (int64_t)tok * p.out_stride_token + (int64_t)h0 * p.out_stride_head;
@@ -85,6 +93,33 @@ hipError_t launch_valu_td(const PrefillParams &p, hipStream_t stream) {
   return hipGetLastError();
 }
 
+template <typename T, int D>
+hipError_t launch_diff_valu_td(const PrefillParams &p, hipStream_t stream) {
+  constexpr int NW = D >= 256 ? 2 : 4;
+  const int gm = p.group > 4 ? 16 : 4;
+  const unsigned gch = (unsigned)((p.group + gm - 1) / gm);
+  const dim3 grid((unsigned)p.num_tokens, (unsigned)p.num_kv_heads * gch);
+  if (gm == 4)
+    hipLaunchKernelGGL((chunked_prefill_valu<T, D, 4, NW, true>), grid, dim3(NW * 64), 0, stream, p);
+  else
+    hipLaunchKernelGGL((chunked_prefill_valu<T, D, 16, NW, true>), grid, dim3(NW * 64), 0, stream,
+                       p);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_diff_valu_t(const PrefillParams &p, hipStream_t stream) {
+  switch (p.head_dim) {
+    case 8: return launch_diff_valu_td<T, 8>(p, stream);
+    case 16: return launch_diff_valu_td<T, 16>(p, stream);
+    case 32: return launch_diff_valu_td<T, 32>(p, stream);
+    case 64: return launch_diff_valu_td<T, 64>(p, stream);
+    case 128: return launch_diff_valu_td<T, 128>(p, stream);
+    case 256: return launch_diff_valu_td<T, 256>(p, stream);
+    default: return hipErrorInvalidValue;
+  }
+}
+
 template <typename T>
 hipError_t launch_valu_t(const PrefillParams &p, hipStream_t stream) {
   switch (p.head_dim) {
@@ -105,6 +140,15 @@ hipError_t launch_prefill_valu(const PrefillParams &p, DType dt, hipStream_t str
     case DType::F32: return launch_valu_t<float>(p, stream);
     case DType::F16: return launch_valu_t<_Float16>(p, stream);
     case DType::BF16: return launch_valu_t<__bf16>(p, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_diff_prefill_valu(const PrefillParams &p, DType dt, hipStream_t stream) {
+  switch (dt) {
+    case DType::F32: return launch_diff_valu_t<float>(p, stream);
+    case DType::F16: return launch_diff_valu_t<_Float16>(p, stream);
+    case DType::BF16: return launch_diff_valu_t<__bf16>(p, stream);
   }
   return hipErrorInvalidValue;
 }

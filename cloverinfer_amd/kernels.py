@@ -747,3 +747,195 @@ def chunked_prefill(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
                       "clv_chunked_prefill_split")
     else:
         _native.check(lib.clv_chunked_prefill(a, _stream(dev)), "clv_chunked_prefill")
+
+
+def _diff_args(lam, norm_weight, norm_eps, out_scale, rows, num_heads, head_dim,
+               dev) -> _native.DiffArgs:
+    a = _native.DiffArgs()
+    if isinstance(lam, torch.Tensor):
+        if lam.device != dev:
+            raise ValueError(f"lam must be on {dev}, found it on {lam.device}")
+        if lam.dtype != torch.float32 or lam.shape not in ((num_heads,), (rows, num_heads)):
+            raise ValueError(f"lam must be a number or a float32 tensor [{num_heads}] or "
+                             f"[{rows}, {num_heads}], got {lam.dtype} {tuple(lam.shape)}")
+        a.lambda_ = lam.data_ptr()
+        a.lambda_stride_row = lam.stride(0) if lam.dim() == 2 else 0
+        a.lambda_stride_head = lam.stride(-1)
+    else:
+        a.lambda_value = float(lam)
+    if norm_weight is not None:
+        if norm_weight.device != dev:
+            raise ValueError(f"norm_weight must be on {dev}, found it on {norm_weight.device}")
+        if norm_weight.dtype != torch.float32 or norm_weight.shape != (head_dim,) \
+                or not norm_weight.is_contiguous():
+            raise ValueError(f"norm_weight must be a contiguous float32 tensor [{head_dim}]")
+        a.norm_weight = norm_weight.data_ptr()
+    a.norm_eps = float(norm_eps)
+    a.out_scale = float(out_scale)
+    return a
+
+
+def _half_scale(scale, q) -> float:
+    """The softmax scale of differential attention: 1/sqrt of a half head for None."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(q.shape[-1] / 2)
+    return scale
+
+
+def differential_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
+                           v_cache: torch.Tensor, block_tables: torch.Tensor,
+                           context_lens: torch.Tensor, block_size: int, max_context_len: int, lam,
+                           norm_weight: torch.Tensor | None = None, norm_eps: float = 1e-5,
+                           out_scale: float = 1.0, scale: float | None = None,
+                           num_waves: int = 0, k_scale=None, v_scale=None) -> None:
+    """Differential attention of one query row per sequence over its paged context.
+
+    Query head h is a pair of half heads: ``q[s, h]`` = q1 | q2, a key row of its
+    kv head k1 | k2 (a ``[.., 2 * heads, head_dim / 2]`` tensor of alternating
+    maps, viewed as ``[.., heads, head_dim]``), and the two softmax maps share
+    the value row of the whole head_dim: a_m = softmax(scale * q_m . K_m^T) V,
+    o = a_1 - lam * a_2, ``out`` = out_scale * o, or with ``norm_weight``
+    (float32 [head_dim]) out_scale * norm_weight * o / sqrt(mean(o^2) +
+    norm_eps). ``lam``: a number, or a float32 tensor [num_heads] or
+    [num_seqs, num_heads]. ``scale`` defaults to 1/sqrt(head_dim / 2). The other
+    arguments are :func:`paged_attention`'s, pools, tables and appends too;
+    fp8 pools need head_dim 128 and block_size >= 16. Key values must be finite.
+
+    Contexts of up to 512 tokens are one launch; longer ones (head_dim 64, 128
+    or 256, block_size >= 4) are split evenly over the chip, over ``num_waves``
+    waves (0 = the device default), and joined.
+    """
+    a = _decode_args(out, q, k_cache, v_cache, block_tables, context_lens, block_size,
+                     max_context_len, _half_scale(scale, q))
+    dev = q.device
+    d = _diff_args(lam, norm_weight, norm_eps, out_scale, a.num_seqs, a.num_heads, a.head_dim, dev)
+    lib = _native.load()
+    stream = _stream(dev)
+    fp8 = k_cache.dtype == FP8
+    ks = vs = None
+    if fp8:
+        ks = kv_scales(k_scale, a.num_kv_heads, dev)
+        vs = kv_scales(v_scale, a.num_kv_heads, dev)
+    nbytes = lib.clv_diff_decode_workspace_bytes(a, fp8, num_waves)
+    # From the caching allocator, as in chunked_prefill.
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _native.check(lib.clv_diff_decode(a, d, ks.data_ptr() if fp8 else None,
+                                      vs.data_ptr() if fp8 else None, num_waves,
+                                      ws.data_ptr() if nbytes else None, nbytes, stream),
+                  "clv_diff_decode")
+
+
+def differential_prefill(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
+                         v_cache: torch.Tensor, block_tables: torch.Tensor,
+                         context_lens: torch.Tensor, query_start_loc: torch.Tensor,
+                         max_query_len: int | None, lam, norm_weight: torch.Tensor | None = None,
+                         norm_eps: float = 1e-5, out_scale: float = 1.0,
+                         scale: float | None = None) -> None:
+    """Differential attention (:func:`differential_attention`) of each
+    sequence's new query rows, causal over its paged context: rows, lengths and
+    ``max_query_len`` as in :func:`chunked_prefill`, ``lam`` a number or a
+    float32 tensor [num_heads] or [num_tokens, num_heads]. fp32/fp16/bf16 pools
+    of the queries' dtype."""
+    scale = _half_scale(scale, q)
+    a = None
+    if max_query_len is not None:
+        a = _filled("fill_prefill_args", _native.PrefillArgs(), out, q, k_cache, v_cache,
+                    block_tables, context_lens, query_start_loc, max_query_len, scale)
+    if a is None:
+        a = _prefill_args(out, q, k_cache, v_cache, block_tables, context_lens, query_start_loc,
+                          max_query_len, scale)
+    dev = q.device
+    d = _diff_args(lam, norm_weight, norm_eps, out_scale, a.num_tokens, a.num_heads, a.head_dim, dev)
+    lib = _native.load()
+    nbytes = lib.clv_diff_prefill_workspace_bytes(a)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _native.check(lib.clv_diff_prefill(a, d, ws.data_ptr() if nbytes else None, nbytes,
+                                       _stream(dev)), "clv_diff_prefill")
+
+
+# advance_block_tables' status (the value it leaves in ``status``).
+TABLES_OK, TABLES_NO_BLOCKS, TABLES_ROW_FULL, TABLES_NO_SLOTS, TABLES_BAD_STATE = range(5)
+
+
+def _tables_args(block_tables, blocks_held, context_lens, new_lens, free_blocks, num_free,
+                 block_size, slot_mapping, query_start_loc, status, reserve, blocks_held_out,
+                 context_lens_out, num_free_out) -> _native.TablesArgs:
+    _require_device(block_tables, blocks_held, context_lens, new_lens, free_blocks, num_free,
+                    slot_mapping, query_start_loc, status, blocks_held_out, context_lens_out,
+                    num_free_out)
+    if block_tables.dtype != torch.int32 or block_tables.dim() != 2 \
+            or not block_tables.is_contiguous():
+        raise ValueError("block_tables must be a contiguous int32 [rows, width] tensor")
+    rows, width = block_tables.shape
+    for name, t, shape in (("blocks_held", blocks_held, (rows,)),
+                           ("context_lens", context_lens, (rows,)),
+                           ("new_lens", new_lens, (rows,)),
+                           ("free_blocks", free_blocks, (free_blocks.shape[0],)),
+                           ("num_free", num_free, (1,)),
+                           ("query_start_loc", query_start_loc, (rows + 1,)),
+                           ("status", status, (1,)),
+                           ("blocks_held_out", blocks_held_out, (rows,)),
+                           ("context_lens_out", context_lens_out, (rows,)),
+                           ("num_free_out", num_free_out, (1,))):
+        if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1 \
+            or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be a contiguous int64 vector")
+    a = _native.TablesArgs()
+    a.block_tables = block_tables.data_ptr()
+    a.blocks_held, a.context_lens = blocks_held.data_ptr(), context_lens.data_ptr()
+    a.new_lens = new_lens.data_ptr()
+    a.free_blocks, a.num_free = free_blocks.data_ptr(), num_free.data_ptr()
+    a.blocks_held_out = blocks_held_out.data_ptr()
+    a.context_lens_out, a.num_free_out = context_lens_out.data_ptr(), num_free_out.data_ptr()
+    a.slot_mapping, a.query_start_loc = slot_mapping.data_ptr(), query_start_loc.data_ptr()
+    a.status = status.data_ptr()
+    a.num_tokens = slot_mapping.shape[0]
+    a.rows, a.width, a.block_size = rows, width, int(block_size)
+    a.num_blocks, a.reserve = free_blocks.shape[0], int(reserve)
+    return a
+
+
+def advance_block_tables(block_tables: torch.Tensor, blocks_held: torch.Tensor,
+                         context_lens: torch.Tensor, new_lens: torch.Tensor,
+                         free_blocks: torch.Tensor, num_free: torch.Tensor, block_size: int,
+                         slot_mapping: torch.Tensor, query_start_loc: torch.Tensor,
+                         status: torch.Tensor, reserve: int = 1,
+                         blocks_held_out: torch.Tensor | None = None,
+                         context_lens_out: torch.Tensor | None = None,
+                         num_free_out: torch.Tensor | None = None) -> None:
+    """One scheduling step of the paged cache, on the GPU (clv_advance_block_tables).
+
+    Row r of ``block_tables`` (int32 [rows, width]) holds ``blocks_held[r]``
+    blocks for ``context_lens[r]`` tokens; ``new_lens[r]`` > 0 tokens join it, 0
+    leaves it, a negative number ends it. ``free_blocks[:num_free]`` is the LIFO
+    stack of free blocks. Ended rows push their blocks, growing rows pop theirs,
+    in row order: the placement of :class:`KVCacheManager` with ``free`` for the
+    ended rows and then ``allocate`` (``reserve`` 1, counted for rows that held
+    nothing) or ``append_slot`` for the growing ones. ``slot_mapping`` (int64)
+    receives the slot of each new token, rows in order, -1 past the last, so it
+    may be longer than the step; ``query_start_loc`` (int32 [rows + 1]) the first
+    new token of every row: what :func:`reshape_and_cache`,
+    :func:`chunked_prefill` and their differential forms read.
+
+    The state is updated in place unless ``_out`` tensors take it (the table's
+    new entries and the pushed blocks are written in place either way; entries
+    past ``blocks_held`` stay as they were). All or nothing: ``status`` (int32
+    [1]) receives TABLES_OK, or TABLES_NO_BLOCKS, TABLES_ROW_FULL (a row needs
+    more than ``width`` blocks), TABLES_NO_SLOTS or TABLES_BAD_STATE, with the
+    state kept, every slot -1 and ``query_start_loc`` 0. Nothing is copied to the
+    host: a step can be captured into a graph with the calls that read it.
+    At most 2048 rows; block_size a power of two.
+    """
+    a = _tables_args(block_tables, blocks_held, context_lens, new_lens, free_blocks, num_free,
+                     block_size, slot_mapping, query_start_loc, status, reserve,
+                     blocks_held if blocks_held_out is None else blocks_held_out,
+                     context_lens if context_lens_out is None else context_lens_out,
+                     num_free if num_free_out is None else num_free_out)
+    dev = block_tables.device
+    lib = _native.load()
+    nbytes = lib.clv_tables_workspace_bytes(a)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _native.check(lib.clv_advance_block_tables(a, ws.data_ptr() if nbytes else None, nbytes,
+                                               _stream(dev)), "clv_advance_block_tables")

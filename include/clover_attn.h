@@ -118,6 +118,78 @@ typedef struct clv_prefill_args {
   float scale;
 } clv_prefill_args;
 
+/*
+ * Differential attention: a query head is a pair of half heads whose softmax
+ * maps share one value of the whole head_dim,
+ *   a_m = softmax_t(scale * q_m.k_m[t]) . V[t]   (m = 1, 2),
+ *   o   = a_1 - lambda * a_2,
+ *   out = out_scale * o                                    (norm_weight null)
+ *   out = out_scale * norm_weight * o / sqrt(mean_d(o^2) + norm_eps)   (else).
+ * Rows of q and of the key pool hold the halves side by side, q_1 | q_2 and
+ * k_1 | k_2 (head_dim / 2 elements each; a [.., 2 * heads, head_dim / 2] tensor
+ * of alternating maps has the same memory), so pools, appends (also the fp8
+ * one) and tables are those of plain attention with the same head_dim. lambda
+ * of (row of q, head) is lambda[row * lambda_stride_row + head *
+ * lambda_stride_head] (a stride of 0 shares it), or lambda_value where lambda
+ * is null. out_scale is 1 - lambda_init of the layer where the norm is used.
+ * Everything between the loads and the rounding of out is fp32.
+ */
+typedef struct clv_diff_args {
+  const float *lambda;
+  int64_t lambda_stride_row, lambda_stride_head; /* elements */
+  const float *norm_weight;                      /* [head_dim] */
+  float lambda_value, norm_eps, out_scale;
+} clv_diff_args;
+
+/*
+ * One scheduling step of the paged cache's bookkeeping, on the GPU: every row
+ * r of a block table brings new_lens[r] tokens (> 0), nothing (0), or ends
+ * (< 0). free_blocks[0, num_free) is the LIFO stack of free blocks, its end on
+ * top.
+ *   - rows that end push their blocks, rows in order, each in table order, and
+ *     are left with 0 blocks and 0 tokens;
+ *   - rows that bring tokens pop blocks (rows in order) until they hold
+ *     ceil((context_lens + new_lens) / block_size), where a row that held none
+ *     counts `reserve` tokens more;
+ *   - slot_mapping[i] becomes the cache slot (block * block_size + offset) of
+ *     the i-th new token, rows in order, -1 past the last one;
+ *     query_start_loc[r] the first new token of row r.
+ * Placement is that of the reference's KVCacheManager (src/core/
+ * memory_manager.py:49-72, 95-121, 134-143) with free() called for the ended
+ * rows and then allocate() (reserve = 1) or append_slot() for the growing ones.
+ * Written: table entries a row gains, the stack entries pushed and left on it,
+ * and the outputs; all else stays as it was (also the entries of rows that
+ * ended: columns at or past blocks_held are not part of the table). The _out
+ * pointers may be the inputs. All or nothing: where status[0] is not
+ * CLV_TABLES_OK the state is kept, query_start_loc is 0 and every slot -1.
+ */
+enum clv_tables_status {
+  CLV_TABLES_OK = 0,
+  CLV_TABLES_NO_BLOCKS = 1, /* the stack has too few blocks                     */
+  CLV_TABLES_ROW_FULL = 2,  /* a row needs more than `width` blocks             */
+  CLV_TABLES_NO_SLOTS = 3,  /* more new tokens than slot_mapping has entries    */
+  CLV_TABLES_BAD_STATE = 4  /* counts or lengths that no sequence of steps makes */
+};
+
+#define CLV_TABLES_MAX_ROWS 2048
+
+typedef struct clv_tables_args {
+  int32_t *block_tables;        /* [rows, width]                  */
+  const int32_t *blocks_held;   /* [rows]                         */
+  const int32_t *context_lens;  /* [rows], before the step        */
+  const int32_t *new_lens;      /* [rows]                         */
+  int32_t *free_blocks;         /* [num_blocks]                   */
+  const int32_t *num_free;      /* [1]                            */
+  int32_t *blocks_held_out;     /* [rows]                         */
+  int32_t *context_lens_out;    /* [rows]                         */
+  int32_t *num_free_out;        /* [1]                            */
+  int64_t *slot_mapping;        /* [num_tokens]                   */
+  int32_t *query_start_loc;     /* [rows + 1]                     */
+  int32_t *status;              /* [1], enum clv_tables_status    */
+  int64_t num_tokens;           /* entries of slot_mapping        */
+  int32_t rows, width, block_size, num_blocks, reserve;
+} clv_tables_args;
+
 /* ABI version of the loaded library (CLV_ABI_VERSION at build time). */
 int clv_abi_version(void);
 
@@ -373,6 +445,45 @@ int clv_chunked_prefill_split(const clv_prefill_args *args, void *workspace,
 /* Workspace bytes of clv_chunked_prefill_split: a function of the argument
  * block's sizes; 0 where the call is not split or the arguments are refused. */
 size_t clv_prefill_workspace_bytes(const clv_prefill_args *args);
+
+/*
+ * Differential decode: clv_paged_decode's call (args: num_heads pairs, head_dim
+ * both halves) with the two maps and their joint of clv_diff_args. k_scales and
+ * v_scales are null, or the pools are fp8 as in clv_paged_decode_fp8 (head_dim
+ * 128, block_size >= 16). Contexts of up to 512 tokens (num_waves <= 0), and
+ * shapes that the balanced decode does not take, are one launch without a
+ * workspace; the rest is a balanced decode over num_waves waves (<= 0: the
+ * device default) and its merge. `workspace`: at least
+ * clv_diff_decode_workspace_bytes() bytes, 256-byte aligned; may be null where
+ * that is 0. A row whose context is empty or unreadable comes out as zeros.
+ * Key values must be finite (each map's score spans the whole key row).
+ * No counterpart in the reference.
+ */
+int clv_diff_decode(const clv_decode_args *args, const clv_diff_args *diff,
+                    const float *k_scales, const float *v_scales, int32_t num_waves,
+                    void *workspace, size_t workspace_bytes, clv_stream_t stream);
+
+size_t clv_diff_decode_workspace_bytes(const clv_decode_args *args, int32_t fp8,
+                                       int32_t num_waves);
+
+/*
+ * Differential attention of each sequence's new rows over its paged context:
+ * clv_chunked_prefill's call with the two maps of clv_diff_args. `workspace` as
+ * above, sized by clv_diff_prefill_workspace_bytes(). No counterpart in the
+ * reference.
+ */
+int clv_diff_prefill(const clv_prefill_args *args, const clv_diff_args *diff, void *workspace,
+                     size_t workspace_bytes, clv_stream_t stream);
+
+size_t clv_diff_prefill_workspace_bytes(const clv_prefill_args *args);
+
+/* One step of the block tables (clv_tables_args). `workspace`: at least
+ * clv_tables_workspace_bytes() bytes, 256-byte aligned; may be null where that
+ * is 0. */
+int clv_advance_block_tables(const clv_tables_args *args, void *workspace,
+                             size_t workspace_bytes, clv_stream_t stream);
+
+size_t clv_tables_workspace_bytes(const clv_tables_args *args);
 
 #ifdef __cplusplus
 } /* extern "C" */
