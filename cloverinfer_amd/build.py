@@ -40,6 +40,7 @@ SOURCES = [
     "cache_ops.hip",
     "decode.hip",
     "decode_stream.hip",
+    "diff_prefill.hip",
     "prefill.hip",
     "prefill_f32.hip",
     "prefill_mfma.hip",

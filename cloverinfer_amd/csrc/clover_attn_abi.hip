@@ -753,6 +753,21 @@ size_t split_bytes(const clv::PrefillParams &p, const clv::PrefillSplitShape &sh
          round256(rows * (size_t)p.head_dim * 4);
 }
 
+clv::PrefillSplit split_workspace(const clv::PrefillSplitShape &sh, void *workspace) {
+  const size_t rows = 2 * (size_t)sh.groups * (size_t)sh.rows;
+  char *ws = (char *)workspace;
+  clv::PrefillSplit sp;
+  sp.groups = sh.groups;
+  sp.desc = ws;
+  ws += round256((size_t)sh.groups * clv::kPrefillDescBytes);
+  sp.ws_m = (float *)ws;
+  ws += round256(rows * 4);
+  sp.ws_l = (float *)ws;
+  ws += round256(rows * 4);
+  sp.ws_o = (float *)ws;
+  return sp;
+}
+
 int launch_prefill(const clv::PrefillParams &p, DType dt, PrefillKernel k,
                    const clv::PrefillSplit *sp, hipStream_t stream) {
   hipError_t err = hipErrorInvalidValue;
@@ -795,17 +810,7 @@ int clv_chunked_prefill_split(const clv_prefill_args *a, void *workspace, size_t
   if (workspace == nullptr || workspace_bytes < split_bytes(p, sh) ||
       ((uintptr_t)workspace & 255u) != 0)
     return CLV_EWORKSPACE;
-  const size_t rows = 2 * (size_t)sh.groups * (size_t)sh.rows;
-  char *ws = (char *)workspace;
-  clv::PrefillSplit sp;
-  sp.groups = sh.groups;
-  sp.desc = ws;
-  ws += round256((size_t)sh.groups * clv::kPrefillDescBytes);
-  sp.ws_m = (float *)ws;
-  ws += round256(rows * 4);
-  sp.ws_l = (float *)ws;
-  ws += round256(rows * 4);
-  sp.ws_o = (float *)ws;
+  const clv::PrefillSplit sp = split_workspace(sh, workspace);
   return launch_prefill(p, dt, k, &sp, (hipStream_t)stream);
 }
 
@@ -904,24 +909,41 @@ int clv_diff_decode(const clv_decode_args *a, const clv_diff_args *d, const floa
 }
 
 size_t clv_diff_prefill_workspace_bytes(const clv_prefill_args *a) {
-  (void)a;
-  return 0;
+  clv::PrefillParams p;
+  if (fill_prefill(a, &p) != CLV_OK || p.num_seqs == 0 || p.num_tokens == 0) return 0;
+  if (!clv::diff_prefill_mfma_covers(p, (DType)a->dtype)) return 0;
+  clv::PrefillSplitShape sh = clv::diff_prefill_split_shape(p);
+  sh.rows *= 2;  // of both maps
+  return sh.groups > 0 ? split_bytes(p, sh) : 0;
 }
 
 int clv_diff_prefill(const clv_prefill_args *a, const clv_diff_args *d, void *workspace,
                      size_t workspace_bytes, clv_stream_t stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   clv::PrefillParams p;
   clv::DiffParams diff;
   int st = fill_prefill(a, &p);
   if (st == CLV_OK) st = fill_diff(d, &diff);
   if (st != CLV_OK || p.num_seqs == 0 || p.num_tokens == 0) return st;
   p.diff = diff;
-  p.group *= 2;  // rows of both maps
-  return clv::launch_diff_prefill_valu(p, (DType)a->dtype, (hipStream_t)stream) == hipSuccess
-             ? CLV_OK
-             : CLV_ELAUNCH;
+  const hipStream_t s = (hipStream_t)stream;
+  const DType dt = (DType)a->dtype;
+  hipError_t err;
+  if (clv::diff_prefill_mfma_covers(p, dt)) {
+    clv::PrefillSplitShape sh = clv::diff_prefill_split_shape(p);
+    sh.rows *= 2;
+    clv::PrefillSplit sp;
+    if (sh.groups > 0) {
+      if (workspace == nullptr || workspace_bytes < split_bytes(p, sh) ||
+          ((uintptr_t)workspace & 255u) != 0)
+        return CLV_EWORKSPACE;
+      sp = split_workspace(sh, workspace);
+    }
+    err = clv::launch_diff_prefill_mfma(p, dt, sh.groups > 0 ? &sp : nullptr, s);
+  } else {
+    p.group *= 2;  // rows of both maps
+    err = clv::launch_diff_prefill_valu(p, dt, s);
+  }
+  return err == hipSuccess ? CLV_OK : CLV_ELAUNCH;
 }
 
 }  // extern "C"

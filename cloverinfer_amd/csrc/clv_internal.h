@@ -206,6 +206,12 @@ hipError_t launch_diff_stream_reduce(const DecodeParams &p, DType dt, hipStream_
 size_t tables_workspace_bytes(const TablesParams &p);
 hipError_t launch_tables(const TablesParams &p, void *workspace, hipStream_t stream);
 hipError_t launch_diff_prefill_valu(const PrefillParams &p, DType dt, hipStream_t stream);
+// The 16-bit MFMA form (p.group: query heads per kv head), its cover and split
+// (rows: pairs of rows).
+bool diff_prefill_mfma_covers(const PrefillParams &p, DType dt);
+PrefillSplitShape diff_prefill_split_shape(const PrefillParams &p);
+hipError_t launch_diff_prefill_mfma(const PrefillParams &p, DType dt, const PrefillSplit *sp,
+                                    hipStream_t stream);
 
 // Whether the MFMA decode kernel covers this shape/dtype.
 bool decode_mfma_supported(DType dt, int head_dim, int block_size);
