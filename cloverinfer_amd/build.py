@@ -41,6 +41,7 @@ SOURCES = [
     "decode.hip",
     "decode_stream.hip",
     "diff_prefill.hip",
+    "diff_prefill_f32.hip",
     "prefill.hip",
     "prefill_f32.hip",
     "prefill_mfma.hip",

@@ -852,6 +852,21 @@ bool diff_single_pass(const clv_decode_args &rows, bool fp8, int32_t num_waves) 
              ceil_div(rows.num_heads / rows.num_kv_heads, 16) > clv::kStreamMaxSegments;
 }
 
+PrefillKernel diff_prefill_kernel(const clv::PrefillParams &p, DType dt) {
+  if (dt == DType::F32)
+    return clv::diff_prefill_f32_covers(p) ? PrefillKernel::kF32 : PrefillKernel::kValu;
+  return clv::diff_prefill_mfma_covers(p, dt) ? PrefillKernel::kMfma : PrefillKernel::kValu;
+}
+
+// As split_shape; rows counts those of both maps.
+clv::PrefillSplitShape diff_split_shape(const clv::PrefillParams &p, PrefillKernel k) {
+  clv::PrefillSplitShape sh = {0, 0};
+  if (k == PrefillKernel::kF32) sh = clv::diff_prefill_f32_split_shape(p);
+  if (k == PrefillKernel::kMfma) sh = clv::diff_prefill_split_shape(p);
+  sh.rows *= 2;
+  return sh;
+}
+
 int32_t diff_waves(bool fp8, int32_t num_waves) {
   return num_waves > 0 ? num_waves : fp8 ? clv_default_num_waves_fp8() : clv_default_num_waves();
 }
@@ -911,9 +926,8 @@ int clv_diff_decode(const clv_decode_args *a, const clv_diff_args *d, const floa
 size_t clv_diff_prefill_workspace_bytes(const clv_prefill_args *a) {
   clv::PrefillParams p;
   if (fill_prefill(a, &p) != CLV_OK || p.num_seqs == 0 || p.num_tokens == 0) return 0;
-  if (!clv::diff_prefill_mfma_covers(p, (DType)a->dtype)) return 0;
-  clv::PrefillSplitShape sh = clv::diff_prefill_split_shape(p);
-  sh.rows *= 2;  // of both maps
+  const clv::PrefillSplitShape sh =
+      diff_split_shape(p, diff_prefill_kernel(p, (DType)a->dtype));
   return sh.groups > 0 ? split_bytes(p, sh) : 0;
 }
 
@@ -927,21 +941,25 @@ int clv_diff_prefill(const clv_prefill_args *a, const clv_diff_args *d, void *wo
   p.diff = diff;
   const hipStream_t s = (hipStream_t)stream;
   const DType dt = (DType)a->dtype;
-  hipError_t err;
-  if (clv::diff_prefill_mfma_covers(p, dt)) {
-    clv::PrefillSplitShape sh = clv::diff_prefill_split_shape(p);
-    sh.rows *= 2;
-    clv::PrefillSplit sp;
-    if (sh.groups > 0) {
-      if (workspace == nullptr || workspace_bytes < split_bytes(p, sh) ||
-          ((uintptr_t)workspace & 255u) != 0)
-        return CLV_EWORKSPACE;
-      sp = split_workspace(sh, workspace);
-    }
-    err = clv::launch_diff_prefill_mfma(p, dt, sh.groups > 0 ? &sp : nullptr, s);
-  } else {
-    p.group *= 2;  // rows of both maps
-    err = clv::launch_diff_prefill_valu(p, dt, s);
+  const PrefillKernel k = diff_prefill_kernel(p, dt);
+  const clv::PrefillSplitShape sh = diff_split_shape(p, k);
+  clv::PrefillSplit split;
+  const clv::PrefillSplit *sp = nullptr;
+  if (sh.groups > 0) {
+    if (workspace == nullptr || workspace_bytes < split_bytes(p, sh) ||
+        ((uintptr_t)workspace & 255u) != 0)
+      return CLV_EWORKSPACE;
+    split = split_workspace(sh, workspace);
+    sp = &split;
+  }
+  hipError_t err = hipErrorInvalidValue;
+  switch (k) {
+    case PrefillKernel::kF32: err = clv::launch_diff_prefill_f32(p, sp, s); break;
+    case PrefillKernel::kMfma: err = clv::launch_diff_prefill_mfma(p, dt, sp, s); break;
+    case PrefillKernel::kValu:
+      p.group *= 2;  // rows of both maps
+      err = clv::launch_diff_prefill_valu(p, dt, s);
+      break;
   }
   return err == hipSuccess ? CLV_OK : CLV_ELAUNCH;
 }

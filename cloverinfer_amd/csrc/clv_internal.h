@@ -212,6 +212,11 @@ bool diff_prefill_mfma_covers(const PrefillParams &p, DType dt);
 PrefillSplitShape diff_prefill_split_shape(const PrefillParams &p);
 hipError_t launch_diff_prefill_mfma(const PrefillParams &p, DType dt, const PrefillSplit *sp,
                                     hipStream_t stream);
+// The fp32 MFMA form, likewise.
+bool diff_prefill_f32_covers(const PrefillParams &p);
+PrefillSplitShape diff_prefill_f32_split_shape(const PrefillParams &p);
+hipError_t launch_diff_prefill_f32(const PrefillParams &p, const PrefillSplit *sp,
+                                   hipStream_t stream);
 
 // Whether the MFMA decode kernel covers this shape/dtype.
 bool decode_mfma_supported(DType dt, int head_dim, int block_size);

@@ -22,9 +22,11 @@
 // SIMD run their softmax and their MFMAs in opposite phases; LDS reads run ahead
 // of the MFMAs they feed; tiles go through a ring of three stages. P.V runs in
 // fp16 for both types: P <= 2^8 keeps 11 bits there (a relative error of 2^-11
-// at most), and bf16 V is converted exactly unless its magnitude reaches 2^16,
-// when the workgroup runs again keeping V in bf16 and P as a bf16 value and its
-// residual. The running maximum is only raised by more than 2^8.
+// at most), and bf16 V is converted exactly unless its magnitude reaches 2^16. An
+// accumulator that is not finite makes the workgroup run its tiles again, in a
+// pass that keeps bf16 V as it is and P as a bf16 value and its residual, with 0
+// in the place of infinities and NaN, which only the rows that see them then take
+// (0 * inf is NaN). The running maximum is only raised by more than 2^8.
 #include "prefill_split.h"
 
 #include <type_traits>
@@ -78,6 +80,34 @@ template <int D> struct SplitCfg {
 // Table width in tokens up to which a call is not split.
 constexpr int kSplitMinTokens = 1024;
 
+// Eight values of V (token `pos`, columns d0 ..) with 0 in the place of NaN and
+// infinities; seen_by[column] remembers the first token with a NaN there,
+// seen_by[D + column] with +inf, seen_by[2 D + column] with -inf.
+template <typename T, int D>
+__device__ __forceinline__ u32x4 finite_v8(u32x4 v, int pos, int d0, int *seen_by) {
+  constexpr uint32_t kInf = __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t x = (v[e / 2] >> (16 * (e % 2))) & 0xffffu;
+    if ((x & kInf) != kInf) continue;
+    const int kind = (x & 0x7fffu) != kInf ? 0 : (x & 0x8000u) == 0 ? 1 : 2;
+    atomicMin(&seen_by[kind * D + d0 + e], pos);
+    v[e / 2] &= 0xffffu << (16 * (1 - e % 2));
+  }
+  return v;
+}
+
+// What a row that sees tokens <= last takes from them in a column, beyond the
+// finite values.
+template <int D>
+__device__ __forceinline__ float seen_v(const int *seen_by, int col, int last) {
+  const float inf = __builtin_inff();
+  float x = seen_by[col] <= last ? __builtin_nanf("") : 0.f;
+  if (seen_by[D + col] <= last) x += inf;
+  if (seen_by[2 * D + col] <= last) x -= inf;
+  return x;
+}
+
 template <typename T, int D, bool SPLIT>
 __global__ void __launch_bounds__(kThreads)
 diff_prefill_mfma(const PrefillArgs args) {
@@ -107,7 +137,8 @@ diff_prefill_mfma(const PrefillArgs args) {
 
   __shared__ __attribute__((aligned(16))) char s_mem[kLdsAll];
   __shared__ __attribute__((aligned(4))) uint8_t sValid[3][kBK];  // 1 = the token is readable
-  __shared__ int sOvf;  // set when a bf16 V value did not fit fp16
+  __shared__ int sBad;  // set when an accumulator is not finite
+  __shared__ int sSeenBy[3 * D];  // exact pass, see finite_v8
   typedef PrefillSched<SplitCfg<D>> Sched;
   __shared__ int s_pre[SPLIT ? kPrefillSplitItems + 1 : 1];
   __shared__ int s_tmp[3 * kWaves];
@@ -232,13 +263,15 @@ diff_prefill_mfma(const PrefillArgs args) {
       vreg[i] = buf_load<u32x4>(make_rsrc_range(vbase0 + boff, nrec), voff);
     }
   };
-  auto store_tile = [&](int buf, auto exact_c) {
+  auto store_tile = [&](int tile, auto exact_c) {
     constexpr bool EXACT = decltype(exact_c)::value;
+    const int buf = tile % 3;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int row = lrow + RPP * i;
       store_vec<u32x4>(&sK[buf * kStage + row * KROW + lchunk * 8], kreg[i]);
       u32x4 v = vreg[i];
+      if constexpr (EXACT) v = finite_v8<T, D>(v, tile * kBK + row, 8 * lchunk, sSeenBy);
       if constexpr (kBf16 && !EXACT) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = bf16x2_to_f16x2(v[e]);
@@ -260,11 +293,12 @@ diff_prefill_mfma(const PrefillArgs args) {
   //   M(g): scores of g, then P.V of g - 1;   V(g): online softmax of g.
   // The waves of the first map run M V, those of the second V M with their
   // softmax one step behind. P.V of g - 1 may read the previous tile. Returns
-  // whether a bf16 V value did not fit fp16 (fast pass only).
+  // whether an accumulator was not finite (fast pass only).
   auto run_tiles = [&](auto exact_c) -> bool {
     constexpr bool EXACT = decltype(exact_c)::value;
     typedef Mfma16x16x32<__bf16> MfB;
-    typedef typename std::conditional<EXACT, typename MfB::op_t, pv_t>::type p_t;
+    constexpr bool TWO = EXACT && kBf16;  // P as two bf16 values
+    typedef typename std::conditional<TWO, typename MfB::op_t, pv_t>::type p_t;
 #pragma unroll
     for (int rt = 0; rt < kRT; ++rt) {
 #pragma unroll
@@ -275,7 +309,7 @@ diff_prefill_mfma(const PrefillArgs args) {
       lsum[rt] = (f32x4){0.f, 0.f, 0.f, 0.f};
     }
     f32x4 sacc[2][kRT];     // scores of the step between M and V
-    p_t pa[kRT], pl[kRT];   // P of the step between V and the next M (pl: exact pass)
+    p_t pa[kRT], pl[kRT];   // P of the step between V and the next M (pl: its residual)
 
     // Scores of step g: sacc[h][rt][e] = S[row 16rt + n16][token 32 (g % HS) + 16h + 4j + e].
     auto qk = [&](int g) {
@@ -312,8 +346,8 @@ diff_prefill_mfma(const PrefillArgs args) {
       __builtin_amdgcn_sched_barrier(0);
     };
     const p_t ones = __builtin_bit_cast(
-        p_t, (u32x4){EXACT ? 0x3f803f80u : 0x3c003c00u, EXACT ? 0x3f803f80u : 0x3c003c00u,
-                     EXACT ? 0x3f803f80u : 0x3c003c00u, EXACT ? 0x3f803f80u : 0x3c003c00u});
+        p_t, (u32x4){TWO ? 0x3f803f80u : 0x3c003c00u, TWO ? 0x3f803f80u : 0x3c003c00u,
+                     TWO ? 0x3f803f80u : 0x3c003c00u, TWO ? 0x3f803f80u : 0x3c003c00u});
     // O += P V for step g.
     auto pv = [&](int g) {
       const uint16_t *vrow = sV + ((g / HS) % 3) * kStage +
@@ -332,7 +366,7 @@ diff_prefill_mfma(const PrefillArgs args) {
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int rt = 0; rt < kRT; ++rt) {
-        if constexpr (!EXACT) {
+        if constexpr (!TWO) {
           lsum[rt] = MfPV::run(pa[rt], ones, lsum[rt]);
         } else {
           lsum[rt] = MfB::run(pa[rt], ones, lsum[rt]);
@@ -347,7 +381,7 @@ diff_prefill_mfma(const PrefillArgs args) {
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int rt = 0; rt < kRT; ++rt) {
-          if constexpr (!EXACT) {
+          if constexpr (!TWO) {
             o[rt][m] = MfPV::run(pa[rt], vb, o[rt][m]);
           } else {
             o[rt][m] = MfB::run(pa[rt], vb, o[rt][m]);
@@ -410,7 +444,7 @@ diff_prefill_mfma(const PrefillArgs args) {
       }
 #pragma unroll
       for (int rt = 0; rt < kRT; ++rt) {
-        if constexpr (!EXACT) {
+        if constexpr (!TWO) {
           pa[rt] = pack8<_Float16>(pf[rt]);
         } else {
           float lo[8];
@@ -427,13 +461,15 @@ diff_prefill_mfma(const PrefillArgs args) {
 
     // Cleared by the fast pass only: a clear in the exact pass could race a
     // slower wave's read of it.
-    if (!EXACT && tid == 0) sOvf = 0;
+    if (!EXACT && tid == 0) sBad = 0;
+    if constexpr (EXACT)
+      for (int i = tid; i < 3 * D; i += kThreads) sSeenBy[i] = 0x7fffffff;
     fetch_blocks(t0);
     if (t0 < te) {
       load_tile(t0);
       fetch_blocks(t0 + 1);
-      __syncthreads();  // sOvf cleared, the previous pass or item done with LDS
-      store_tile(t0 % 3, exact_c);
+      __syncthreads();  // sBad or sSeenBy set, the previous pass or item done with LDS
+      store_tile(t0, exact_c);
     }
     __syncthreads();
 
@@ -444,7 +480,7 @@ diff_prefill_mfma(const PrefillArgs args) {
         if (tile + 1 < te) {
           load_tile(tile + 1);
           fetch_blocks(tile + 2);
-          store_tile((tile + 1) % 3, exact_c);
+          store_tile(tile + 1, exact_c);
         }
         __syncthreads();
       }
@@ -472,7 +508,7 @@ diff_prefill_mfma(const PrefillArgs args) {
         if (!lag) softmax(g + HS - 1, full);
         full_prev = full;
 
-        if (more) store_tile((tile + 1) % 3, exact_c);
+        if (more) store_tile(tile + 1, exact_c);
         __syncthreads();
       }
       if (t0 < te) {
@@ -480,9 +516,9 @@ diff_prefill_mfma(const PrefillArgs args) {
         pv(HS * te - 1);
       }
     }
-    if constexpr (kBf16 && !EXACT) {
-      // A V value that did not fit fp16 became an infinity, and with it (0 * inf
-      // included) accumulators of every row of its step infinite or NaN.
+    if constexpr (!EXACT) {
+      // A V value that is infinite or NaN (in fp16, for bf16) makes accumulators
+      // of every row of its step infinite or NaN, hidden ones (0 * inf) included.
       float acc = 0.f;
 #pragma unroll
       for (int rt = 0; rt < kRT; ++rt)
@@ -490,15 +526,23 @@ diff_prefill_mfma(const PrefillArgs args) {
         for (int m = 0; m < CH; ++m)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc += o[rt][m][e] * 0.f;
-      if (__any(acc != 0.f)) sOvf = 1;  // x * 0 is 0 for every finite x
+      if (__any(acc != 0.f)) sBad = 1;  // x * 0 is 0 for every finite x
     }
-    __syncthreads();  // sOvf final; LDS free for a second pass
-    return kBf16 && !EXACT && sOvf != 0;
+    __syncthreads();  // sBad final; LDS free for a second pass
+    return !EXACT && sBad != 0;
   };
 
-  const bool overflow = run_tiles(std::false_type{});
-  if constexpr (kBf16) {
-    if (overflow) run_tiles(std::true_type{});
+  if (run_tiles(std::false_type{})) {
+    run_tiles(std::true_type{});
+#pragma unroll
+    for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int last = __shfl(lim[rt], 4 * j + e, 64);
+#pragma unroll
+        for (int m = 0; m < CH; ++m) o[rt][m][e] += seen_v<D>(sSeenBy, 16 * m + n16, last);
+      }
+    __syncthreads();  // sSeenBy is set anew by the next pass
   }
 
   // ---- join the maps of rows wave_row0 + 16rt + 4j + e and store them, or
@@ -576,101 +620,9 @@ diff_prefill_mfma(const PrefillArgs args) {
   }
   if (t1 == nt && it.qt == ar1.n_qtiles - 1 && it.q_hi < n_new)
     prefill_nan_tail<T, D, kThreads>(ar1.p, it);
-  // The pairs have been read, and every wave has read sOvf, before the next
+  // The pairs have been read, and every wave has read sBad, before the next
   // item writes either.
   if constexpr (SPLIT) __syncthreads();
-  }
-}
-
-// Merges the partials of the items that the split cut, and joins their maps:
-// workgroup (w, y) takes kChunk rows of the item that group w begins and does
-// not finish, D / 4 lanes a row. Four partials of each map are loaded together.
-template <typename T, int D>
-__global__ void __launch_bounds__(256)
-diff_prefill_merge(const PrefillArgs args) {
-  constexpr int kPairs = Shape<D>::kPairs;
-  constexpr int kChunk = 16;
-  constexpr int LPR = D / 4;
-  constexpr int RPP = 256 / LPR;
-  const PrefillParams &p = args.p;
-  const PrefillSplit &sp = args.sp;
-  const PrefillDesc *desc = (const PrefillDesc *)sp.desc;
-  const int w = blockIdx.x;
-  const int lane = threadIdx.x & 63;
-  const int32_t cont0 = desc[min(w + 1 + lane, sp.groups - 1)].cont;
-  const PrefillDesc d = desc[w];
-  const int r_end = min(d.rows, (int)(blockIdx.y + 1) * kChunk);
-  if ((int)blockIdx.y * kChunk >= r_end) return;
-  int n = 1;
-  for (int b = w + 1; b < sp.groups; b += 64) {
-    const int32_t c = b == w + 1 ? cont0 : desc[min(b + lane, sp.groups - 1)].cont;
-    const uint64_t ends = __ballot(b + lane < sp.groups && c == 2);
-    if (ends != 0) {
-      n = b - w + __builtin_ctzll(ends) + 1;
-      break;
-    }
-  }
-  const int G = p.group;
-  const int sub = threadIdx.x % LPR;
-  const float c = fmaxf(fabsf(p.scale_log2), 0x1p-126f);
-  for (int r = blockIdx.y * kChunk + threadIdx.x / LPR; r < r_end; r += RPP) {
-    f32x4 a[2];
-#pragma unroll
-    for (int map = 0; map < 2; ++map) {
-      auto row_of = [&](int k) {  // row of partial k in the workspace
-        return ((int64_t)(k == 0 ? 2 * w + 1 : 2 * (w + k)) * 2 + map) * kPairs + r;
-      };
-      auto load4 = [&](int k0, f32x4 (&v)[4]) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          v[u] = load_vec<f32x4>(sp.ws_o + row_of(min(k0 + u, n - 1)) * D + 4 * sub);
-      };
-      const float m0 = sub < n ? sp.ws_m[row_of(sub)] : kNegInf;
-      const float l0 = sub < n ? sp.ws_l[row_of(sub)] : 0.f;
-      f32x4 v[4];
-      load4(0, v);
-      float M = m0;
-      for (int k = sub + LPR; k < n; k += LPR) M = fmaxf(M, sp.ws_m[row_of(k)]);
-#pragma unroll
-      for (int off = 1; off < LPR; off <<= 1) M = fmaxf(M, __shfl_xor(M, off, LPR));
-      const float Msub = M == kNegInf ? 0.f : M;
-      float L = 0.f;
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-      for (int k0 = 0; k0 < n; k0 += LPR) {
-        const int cnt = min(LPR, n - k0);
-        float wk = 0.f;
-        if (sub < cnt) {
-          wk = fast_exp2(((k0 == 0 ? m0 : sp.ws_m[row_of(k0 + sub)]) - Msub) * c);
-          L += (k0 == 0 ? l0 : sp.ws_l[row_of(k0 + sub)]) * wk;
-        }
-        for (int k = 0; k < cnt; k += 4) {
-          if (k0 + k > 0) load4(k0 + k, v);
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const float f = __shfl(wk, min(k + u, LPR - 1), LPR);
-            if (k + u < cnt) acc += v[u] * f;
-          }
-        }
-      }
-#pragma unroll
-      for (int off = 1; off < LPR; off <<= 1) L += __shfl_xor(L, off, LPR);
-      a[map] = acc * (L > 0.f ? 1.f / L : 0.f);
-    }
-    const int tok = r / G, head = d.kvh * G + r % G;
-    const f32x4 o = a[0] - a[1] * diff_lambda(p.diff, d.row0 + tok, head);
-    float ss = (o[0] * o[0] + o[1] * o[1]) + (o[2] * o[2] + o[3] * o[3]);
-#pragma unroll
-    for (int off = 1; off < LPR; off <<= 1) ss += __shfl_xor(ss, off, LPR);
-    const float f =
-        d.q0 + tok >= p.max_query_len ? __builtin_nanf("") : diff_factor(p.diff, ss, D);
-    f32x4 res = o * f;
-    if (p.diff.weight != nullptr) res *= load_vec<f32x4>(p.diff.weight + 4 * sub);
-    T *dst = (T *)p.out + (int64_t)(d.row0 + tok) * p.out_stride_token +
-             (int64_t)head * p.out_stride_head + 4 * sub;
-    uint32_t h[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) h[e] = __builtin_bit_cast(uint16_t, (T)res[e]);
-    store_vec<u32x2>(dst, (u32x2){h[0] | (h[1] << 16), h[2] | (h[3] << 16)});
   }
 }
 
@@ -688,8 +640,9 @@ hipError_t launch_td(const PrefillParams &p, const PrefillSplit *sp, hipStream_t
     args.sp = *sp;
     hipLaunchKernelGGL((diff_prefill_mfma<T, D, true>), dim3((unsigned)sp->groups), dim3(kThreads),
                        0, stream, args);
-    hipLaunchKernelGGL((diff_prefill_merge<T, D>), dim3((unsigned)sp->groups, kPairs / 16),
-                       dim3(256), 0, stream, args);
+    hipLaunchKernelGGL((diff_prefill_merge<T, D, kPairs>),
+                       dim3((unsigned)sp->groups, kPairs / kDiffMergeRows), dim3(256), 0, stream,
+                       args);
     return hipGetLastError();
   }
   args.total = (int)total;

@@ -365,6 +365,39 @@ def test_prefill_large_bf16_values(d, cached):
     _prefill([cached, 20], [40, 30], 8, 2, d, torch.bfloat16, value_scale=1e5)
 
 
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("pool", ["k", "v"])
+@pytest.mark.parametrize("cached", [0, 1500])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prefill_hidden_values_stay_hidden(dtype, d, cached, pool, value):
+    """A key or value that is not finite reaches no row that does not see its
+    token; in V it reaches only its own column of those that do."""
+    hq, hkv, n, bad = 4, 2, 40, 13
+    ctx = [cached + n, 20]
+    k, v, tables = make_paged_kv(2, ctx, hkv, d, 16, dtype)
+    q = torch.randn(n + 20, hq, d, generator=torch.Generator().manual_seed(2)).to(dtype)
+    kk = [_gathered(k, tables[s], ctx[s], 16) for s in range(2)]
+    vv = [_gathered(v, tables[s], ctx[s], 16) for s in range(2)]
+    pos, col = cached + bad, d - 3
+    block, offset = tables[0][pos // 16], pos % 16
+    (k if pool == "k" else v)[block, offset, 1, col] = value
+    out = torch.zeros_like(q, device=DEV)
+    kernels.differential_prefill(out, q.to(DEV), k.to(DEV), v.to(DEV), padded_tables(tables).to(DEV),
+                                 torch.tensor(ctx, dtype=torch.int32, device=DEV),
+                                 torch.tensor([0, n, n + 20], dtype=torch.int32, device=DEV), n, 0.3)
+    out = out.cpu()
+    clean = od.rows(q[:n], kk[0], vv[0], [cached + i + 1 for i in range(n)], 0.3)
+    if pool == "v":
+        assert not torch.isfinite(out[bad:n, 2:, col]).any()
+        out[bad:n, 2:, col] = clean["out"][bad:, 2:, col].to(dtype)
+    else:  # those rows' heads are all not finite, or all the value's limit
+        out[bad:n, 2:] = clean["out"][bad:, 2:].to(dtype)
+    _check(out[:n], clean, dtype, PREFILL_BITS[dtype], "rows of the sequence")
+    other = od.rows(q[n:], kk[1], vv[1], [i + 1 for i in range(20)], 0.3)
+    _check(out[n:], other, dtype, PREFILL_BITS[dtype], "the other sequence")
+
+
 def test_prefill_one_row_equals_decode():
     """A chunk of one row per sequence is the decode's call."""
     ctx, hq, hkv, d, dtype = [1, 700, 33, 2000], 14, 2, 256, torch.float32
