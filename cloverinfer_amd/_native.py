@@ -230,10 +230,7 @@ SIGNATURES = {
         [ctypes.POINTER(PrefillArgs), ctypes.POINTER(DiffArgs), _c_ptr, ctypes.c_size_t, _c_ptr],
     ),
     "clv_diff_prefill_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PrefillArgs)]),
-    "clv_advance_block_tables": (
-        ctypes.c_int, [ctypes.POINTER(TablesArgs), _c_ptr, ctypes.c_size_t, _c_ptr],
-    ),
-    "clv_tables_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(TablesArgs)]),
+    "clv_advance_block_tables": (ctypes.c_int, [ctypes.POINTER(TablesArgs), _c_ptr]),
 }
 
 _lock = threading.Lock()

@@ -828,6 +828,12 @@ int fill_diff(const clv_diff_args *d, clv::DiffParams *out) {
   return CLV_OK;
 }
 
+// Least steps of a group of the balanced differential decode.
+#ifndef CLV_DIFF_MIN_STEPS
+#define CLV_DIFF_MIN_STEPS 4
+#endif
+constexpr int32_t kDiffMinSteps = CLV_DIFF_MIN_STEPS;
+
 // `a` with the rows of both maps as its heads.
 int diff_rows(const clv_decode_args *a, clv_decode_args *rows) {
   if (a == nullptr || a->num_heads <= 0 || a->num_heads > (1 << 20) || a->num_kv_heads <= 0 ||
@@ -914,6 +920,7 @@ int clv_diff_decode(const clv_decode_args *a, const clv_diff_args *d, const floa
   st = fill_balanced(&r, diff_waves(fp8, num_waves), workspace, workspace_bytes, &p, true);
   if (st != CLV_OK || p.num_seqs == 0) return st;
   p.diff = diff;
+  p.stream_min_steps = kDiffMinSteps;
   if (fp8) {
     p.kv_fp8 = 1;
     p.k_scales = k_scales;
@@ -982,6 +989,20 @@ int fill_tables(const clv_tables_args *a, clv::TablesParams *p) {
   if (a->rows > 0 && (!a->blocks_held || !a->context_lens || !a->new_lens || !a->blocks_held_out ||
                       !a->context_lens_out || (a->width > 0 && !a->block_tables)))
     return CLV_EINVAL;
+  // An output is its own input or apart from all of them: the state is read by
+  // many workgroups while it is written.
+  const struct {
+    const int32_t *in, *out;
+    int64_t n;
+  } state[4] = {{a->blocks_held, a->blocks_held_out, a->rows},
+                {a->context_lens, a->context_lens_out, a->rows},
+                {a->num_free, a->num_free_out, 1},
+                {a->new_lens, nullptr, a->rows}};
+  for (const auto &o : state)
+    for (const auto &i : state)
+      if (o.out != nullptr && i.in != nullptr && o.out < i.in + i.n && i.in < o.out + o.n &&
+          !(&o == &i && o.out == o.in))
+        return CLV_EINVAL;
   *p = clv::TablesParams{a->block_tables,     a->blocks_held,      a->context_lens,
                          a->new_lens,         a->free_blocks,      a->num_free,
                          a->blocks_held_out,  a->context_lens_out, a->num_free_out,
@@ -995,21 +1016,11 @@ int fill_tables(const clv_tables_args *a, clv::TablesParams *p) {
 
 extern "C" {
 
-size_t clv_tables_workspace_bytes(const clv_tables_args *a) {
-  clv::TablesParams p;
-  return fill_tables(a, &p) == CLV_OK ? clv::tables_workspace_bytes(p) : 0;
-}
-
-int clv_advance_block_tables(const clv_tables_args *a, void *workspace, size_t workspace_bytes,
-                             clv_stream_t stream) {
+int clv_advance_block_tables(const clv_tables_args *a, clv_stream_t stream) {
   clv::TablesParams p;
   const int st = fill_tables(a, &p);
   if (st != CLV_OK) return st;
-  const size_t need = clv::tables_workspace_bytes(p);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 255u)))
-    return CLV_EWORKSPACE;
-  return clv::launch_tables(p, workspace, (hipStream_t)stream) == hipSuccess ? CLV_OK
-                                                                             : CLV_ELAUNCH;
+  return clv::launch_tables(p, (hipStream_t)stream) == hipSuccess ? CLV_OK : CLV_ELAUNCH;
 }
 
 }  // extern "C"

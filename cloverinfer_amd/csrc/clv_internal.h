@@ -52,6 +52,7 @@ struct DecodeParams {
   int32_t head_group;     // kv heads read together (1, 2 or 4; divides num_kv_heads)
   int32_t stream_depth;   // steps of loads each wave keeps in flight
   int32_t stream_run_cost;  // phantom steps charged for each segment start (see decode_stream.hip)
+  int32_t stream_min_steps; // differential decode: least steps per group
   int32_t num_segments;   // num_seqs * (num_kv_heads / head_group) * n_gchunks
   int32_t *seg_prefix;    // [num_segments + 1] exclusive prefix of steps per segment
   // Split by dispatch slot (see StreamSplit in decode_stream.hip): with
@@ -202,9 +203,7 @@ hipError_t launch_diff_decode_mfma(const DecodeParams &p, DType dt, hipStream_t 
 hipError_t launch_diff_decode_valu(const DecodeParams &p, DType dt, hipStream_t stream);
 hipError_t launch_diff_decode_stream(const DecodeParams &p, DType dt, hipStream_t stream);
 hipError_t launch_diff_stream_reduce(const DecodeParams &p, DType dt, hipStream_t stream);
-// A step of the block tables; workspace: tables_workspace_bytes (0: none).
-size_t tables_workspace_bytes(const TablesParams &p);
-hipError_t launch_tables(const TablesParams &p, void *workspace, hipStream_t stream);
+hipError_t launch_tables(const TablesParams &p, hipStream_t stream);
 hipError_t launch_diff_prefill_valu(const PrefillParams &p, DType dt, hipStream_t stream);
 // The 16-bit MFMA form (p.group: query heads per kv head), its cover and split
 // (rows: pairs of rows).

@@ -771,16 +771,15 @@ struct StreamWave<float, D, UNI, false> {
 // a decode over a context can take one more token after its partials are
 // written. The score is xm = (sum over the wave of xdot) * xscale, summed
 // here after the rows' loads are issued so that its shuffles overlap them.
-// The merged row's element lane + 64 e comes back in res[e], in wave wv = 0 of
-// the NW (true; the others hold no result).
-template <int D, int NW, bool X = false>
-__device__ __forceinline__ bool lse_merge_row(const float *m, const float *l, const float *c,
-                                              int64_t ms, int64_t cs, int n, int wv, float *smem,
-                                              float (&res)[(D + 63) / 64], float xdot = 0.f,
-                                              float xscale = 0.f, const float *xv = nullptr) {
+template <typename T, int D, int NW, bool X = false>
+__device__ __forceinline__ void lse_merge(const float *m, const float *l, const float *c,
+                                          int64_t ms, int64_t cs, int n, T *dst, float *smem,
+                                          float xdot = 0.f, float xscale = 0.f,
+                                          const float *xv = nullptr) {
   constexpr int EPL = (D + 63) / 64;
   constexpr int R = NW > 1 ? 16 : 8;
   const int lane = threadIdx.x & 63;
+  const int wv = NW > 1 ? (int)(threadIdx.x >> 6) : 0;
   const int C = NW > 1 ? max(1, min(64, (n + NW - 1) / NW)) : 64;
   // The row's max needs every m_i; the first chunk's (m, l) and its first
   // R context rows are loaded together, before any reduction, so that a
@@ -852,7 +851,7 @@ __device__ __forceinline__ bool lse_merge_row(const float *m, const float *l, co
     for (int e = 0; e < EPL; ++e)
       if (lane + 64 * e < D) sa[wv * D + lane + 64 * e] = acc[e];
     __syncthreads();
-    if (wv != 0) return false;
+    if (wv != 0) return;
     L = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) L += sl[w];
@@ -872,25 +871,8 @@ __device__ __forceinline__ bool lse_merge_row(const float *m, const float *l, co
   }
   const float inv = 1.f / fmaxf(L, 1e-12f);
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) res[e] = acc[e] * inv;
-  return true;
-}
-
-// lse_merge_row with the row written to dst.
-template <typename T, int D, int NW, bool X = false>
-__device__ __forceinline__ void lse_merge(const float *m, const float *l, const float *c,
-                                          int64_t ms, int64_t cs, int n, T *dst, float *smem,
-                                          float xdot = 0.f, float xscale = 0.f,
-                                          const float *xv = nullptr) {
-  constexpr int EPL = (D + 63) / 64;
-  const int lane = threadIdx.x & 63;
-  float res[EPL];
-  if (!lse_merge_row<D, NW, X>(m, l, c, ms, cs, n, NW > 1 ? (int)(threadIdx.x >> 6) : 0, smem, res,
-                               xdot, xscale, xv))
-    return;
-#pragma unroll
   for (int e = 0; e < EPL; ++e)
-    if (lane + 64 * e < D) dst[lane + 64 * e] = from_f32<T>(res[e]);
+    if (lane + 64 * e < D) dst[lane + 64 * e] = from_f32<T>(acc[e] * inv);
 }
 
 }  // namespace clv

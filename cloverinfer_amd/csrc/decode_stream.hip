@@ -119,6 +119,17 @@ struct StreamSplit {
   }
 };
 
+// Groups that share N steps: at most one per step, so that every group owns at
+// least one and each segment's partials come from consecutive groups. DIFF: at
+// least stream_min_steps each, as a group's partial (the rows of both maps) takes
+// as many bytes to write and merge as a few steps take to read.
+template <bool DIFF>
+__device__ __forceinline__ int64_t used_groups(const DecodeParams &p, int64_t N) {
+  const int64_t all = p.num_waves / p.head_group;
+  if constexpr (DIFF) return min(all, (N + p.stream_min_steps - 1) / p.stream_min_steps);
+  return min(all, N);
+}
+
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // In-place exclusive prefix sum of buf[0, n) by the 256 threads of the
@@ -210,9 +221,7 @@ paged_decode_stream(const DecodeParams p, const int32_t *__restrict__ tables,
   }
   __syncthreads();
   const int64_t N = block_exclusive_scan(s_seg, nseg, s_tmp);
-  // At most one group per step, so that every group owns at least one step
-  // and each segment's partials come from consecutive groups.
-  const int64_t W = min((int64_t)(p.num_waves / HG), N);
+  const int64_t W = used_groups<DIFF>(p, N);
   if (!PART && blockIdx.x == 0) {
     for (int i = threadIdx.x; i <= nseg; i += kThreads) seg_prefix[i] = s_seg[i];
   }
@@ -423,6 +432,7 @@ paged_decode_stream(const DecodeParams p, const int32_t *__restrict__ tables,
 // The partials of one row (query row `gall` of kv head kvh of sequence s) that
 // the stream kernel left: their count n, and the workspace row of the first
 // (the others follow at a stride of 16 * head_group rows).
+template <bool DIFF>
 __device__ __forceinline__ int64_t row_partials(const DecodeParams &p, int s, int kvh, int gall,
                                                 int &n) {
   const int HG = p.head_group;
@@ -445,7 +455,7 @@ __device__ __forceinline__ int64_t row_partials(const DecodeParams &p, int s, in
     b = (int)(uint32_t)(ab >> 32);
   }
   const int64_t N = n_total;
-  const int64_t W = min((int64_t)(p.num_waves / HG), N);
+  const int64_t W = used_groups<DIFF>(p, N);
   int w0 = 0;
   n = 0;
   if (b > a) {
@@ -499,7 +509,7 @@ __global__ void __launch_bounds__(NW > 1 ? NW * 64 : 256) stream_reduce(const De
   }
   const int HG = p.head_group;
   int n;
-  const int64_t row0 = row_partials(p, s, kvh, gall, n);
+  const int64_t row0 = row_partials<false>(p, s, kvh, gall, n);
   T *dst = (T *)p.out + (int64_t)s * p.out_stride_seq + (int64_t)h * p.out_stride_head;
   if constexpr (!NEW) {
     lse_merge<T, D, NW>(p.ws_m + row0, p.ws_l + row0, p.ws_o + row0 * D, 16 * HG, 16 * HG * D, n,
@@ -541,18 +551,23 @@ __global__ void __launch_bounds__(NW > 1 ? NW * 64 : 256) stream_reduce(const De
 
 // Merge of a differential decode: NW waves per row of a map, so 2 NW per
 // (sequence, query head); the first map's wave joins the pair, normalises and
-// writes it. A workgroup holds two pairs at NW = 1, one otherwise.
+// writes it. A workgroup holds two pairs at NW = 1, one otherwise. The rule is
+// lse_merge's; a lane holds D / 64 consecutive columns, so a row is one load
+// instruction, and the first R rows are loaded with the row maxima and sums.
 template <typename T, int D, int NW>
 __global__ void __launch_bounds__(NW > 1 ? 2 * NW * 64 : 256)
 diff_stream_reduce(const DecodeParams p) {
-  constexpr int EPL = (D + 63) / 64;
+  constexpr int EPL = D / 64;
+  typedef float vec_t __attribute__((ext_vector_type(EPL)));
   constexpr int PAIRS = NW > 1 ? 1 : 2;
-  __shared__ float smem[NW > 1 ? 2 : 1][NW > 1 ? NW * (D + 1) : 1];
-  __shared__ float s_second[PAIRS][D];
+  constexpr int R = NW > 1 ? 16 : 8;
+  __shared__ float s_l[2 * NW];
+  __shared__ __attribute__((aligned(16))) float s_o[NW > 1 ? 2 * NW : PAIRS][D];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   const int slot = NW > 1 ? 0 : wave >> 1;
   const int map = NW > 1 ? wave / NW : wave & 1;
+  const int wv = NW > 1 ? wave % NW : 0;
   const int heads = p.num_heads / 2;
   const int64_t idx = (int64_t)blockIdx.x * PAIRS + slot;
   const bool any = idx < (int64_t)p.num_seqs * heads;
@@ -560,34 +575,88 @@ diff_stream_reduce(const DecodeParams p) {
   const int h = any ? (int)(idx - (int64_t)s * heads) : 0;
   const int kvh = h / (p.group / 2);
   int n;
-  const int64_t row0 = row_partials(p, s, kvh, 2 * h - kvh * p.group + map, n);
-  const int HG = p.head_group;
-  float a[EPL];
-  const bool mine = lse_merge_row<D, NW>(p.ws_m + row0, p.ws_l + row0, p.ws_o + row0 * D, 16 * HG,
-                                         16 * HG * D, n, NW > 1 ? wave % NW : 0,
-                                         smem[NW > 1 ? map : 0], a);
-  if (mine && map == 1)
+  const int64_t row0 = row_partials<true>(p, s, kvh, 2 * h - kvh * p.group + map, n);
+  const int64_t rs = 16 * p.head_group;  // rows between a row's partials
+  const float *m = p.ws_m + row0, *l = p.ws_l + row0, *c = p.ws_o + row0 * D + lane * EPL;
+  // Wave wv takes chunks of C partials; each lane weighs one of a chunk.
+  const int C = NW > 1 ? max(1, min(64, (n + NW - 1) / NW)) : 64;
+  const int base0 = C * wv;
+  const int cnt0 = max(0, min(C, n - base0));
+  float m0 = kNegInf, l0 = 0.f;
+  if (lane < cnt0) {
+    m0 = m[(base0 + lane) * rs];
+    l0 = l[(base0 + lane) * rs];
+  }
+  vec_t v[R];
 #pragma unroll
-    for (int e = 0; e < EPL; ++e)
-      if (lane + 64 * e < D) s_second[slot][lane + 64 * e] = a[e];
-  __syncthreads();
-  if (!mine || map == 1 || !any) return;
-  const float lam = diff_lambda(p.diff, s, h);
+  for (int u = 0; u < R; ++u)
+    v[u] = u < cnt0 ? load_vec<vec_t>(c + (base0 + u) * rs * D) : (vec_t)(0.f);
+  float M = m0;
+  for (int i = lane; i < n; i += 64)
+    if (i < base0 || i >= base0 + cnt0) M = fmaxf(M, m[i * rs]);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) M = fmaxf(M, shfl_xor(M, off));
+  const float Msub = (M == kNegInf) ? 0.f : M;
+  float L = 0.f;
+  vec_t a = (vec_t)(0.f);
+  for (int base = base0; base < n; base += C * NW) {
+    const int cnt = min(C, n - base);
+    float wl = 0.f;
+    if (base == base0) {
+      if (lane < cnt) wl = l0 * fast_exp2((m0 - Msub) * kLog2e);
+    } else if (lane < cnt) {
+      wl = l[(base + lane) * rs] * fast_exp2((m[(base + lane) * rs] - Msub) * kLog2e);
+    }
+    L += wl;
+    for (int k = 0; k < cnt; k += R) {
+      if (base != base0 || k != 0) {
+#pragma unroll
+        for (int u = 0; u < R; ++u)
+          v[u] = k + u < cnt ? load_vec<vec_t>(c + (base + k + u) * rs * D) : (vec_t)(0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < R; ++u)
+        a += v[u] * __builtin_bit_cast(float, __builtin_amdgcn_readlane(
+                                                  __builtin_bit_cast(int, wl), min(k + u, 63)));
+    }
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) L += shfl_xor(L, off);
+  if constexpr (NW > 1) {
+    if (lane == 0) s_l[wave] = L;
+    store_vec<vec_t>(&s_o[wave][lane * EPL], a);
+    __syncthreads();
+    if (wave != 0) return;
+    vec_t both[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float sum = 0.f;
+      vec_t t = (vec_t)(0.f);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        sum += s_l[k * NW + w];
+        t += load_vec<vec_t>(&s_o[k * NW + w][lane * EPL]);
+      }
+      both[k] = t * (1.f / fmaxf(sum, 1e-12f));
+    }
+    a = both[0] - both[1] * diff_lambda(p.diff, s, h);
+  } else {
+    a *= 1.f / fmaxf(L, 1e-12f);
+    if (map == 1) store_vec<vec_t>(&s_o[slot][lane * EPL], a);
+    __syncthreads();
+    if (map == 1 || !any) return;
+    a -= load_vec<vec_t>(&s_o[slot][lane * EPL]) * diff_lambda(p.diff, s, h);
+  }
   float ss = 0.f;
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) {
-    a[e] = lane + 64 * e < D ? a[e] - lam * s_second[slot][lane + 64 * e] : 0.f;
-    ss += a[e] * a[e];
-  }
+  for (int e = 0; e < EPL; ++e) ss += a[e] * a[e];
 #pragma unroll
   for (int off = 32; off >= 1; off >>= 1) ss += shfl_xor(ss, off);
-  const float f = diff_factor(p.diff, ss, D);
-  T *dst = (T *)p.out + (int64_t)s * p.out_stride_seq + (int64_t)h * p.out_stride_head;
-#pragma unroll
-  for (int e = 0; e < EPL; ++e) {
-    const int d = lane + 64 * e;
-    if (d < D) dst[d] = from_f32<T>(a[e] * (p.diff.weight != nullptr ? f * p.diff.weight[d] : f));
-  }
+  a *= diff_factor(p.diff, ss, D);
+  if (p.diff.weight != nullptr) a *= load_vec<vec_t>(p.diff.weight + lane * EPL);
+  typedef T out_t __attribute__((ext_vector_type(EPL)));
+  store_vec<out_t>((T *)p.out + (int64_t)s * p.out_stride_seq + (int64_t)h * p.out_stride_head +
+                       lane * EPL, __builtin_convertvector(a, out_t));
 }
 
 template <typename T, int D, int DEPTH>

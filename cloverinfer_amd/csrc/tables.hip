@@ -20,39 +20,34 @@
 // that ended stay as they were.)
 //
 // A step moves a few KB to a few MB, so it is bound by launch and memory
-// latency. Small steps run in one workgroup: it scans the rows (its copy of
-// the state in LDS lets the state be written in place), then serves entries
-// and slots from LDS. Larger ones run a second launch over the chip.
+// latency: a chain of one read of the rows, a scan, a search in LDS, one read of
+// a table or stack entry, one write. Every workgroup scans the rows itself
+// rather than wait for a launch that does, and takes an even share of the step's
+// slots, entries and pushed blocks.
 #include "clover_attn.h"
 #include "clv_device.h"
 
 namespace clv {
 namespace {
 
-constexpr int kScanThreads = 1024;
-constexpr int kFillThreads = 256;
+constexpr int kRun = 4;  // consecutive slots (two 16-byte stores) or pushed blocks of a thread
 
-// A step's rows: exclusive prefix sums [rows + 1], and the state before it [rows].
+// A step's rows in LDS: exclusive prefix sums [rows + 1], and the state before
+// it [rows].
 struct StepRows {
   int32_t *tok, *take, *gone;
   int32_t *len, *held;
+  __device__ __forceinline__ StepRows(int32_t *base, int rows)
+      : tok(base), take(tok + rows + 1), gone(take + rows + 1), len(gone + rows + 1),
+        held(len + rows) {}
 };
 
-__device__ __host__ __forceinline__ StepRows step_rows(int32_t *base, int rows) {
-  StepRows s;
-  s.tok = base;
-  s.take = s.tok + rows + 1;
-  s.gone = s.take + rows + 1;
-  s.len = s.gone + rows + 1;
-  s.held = s.len + rows;
-  return s;
-}
+size_t rows_bytes(int rows) { return (size_t)(5 * rows + 3) * 4; }
 
 // What a step does in all.
 struct StepTotals {
   int32_t tokens, take, gone;
   int32_t num_free;  // before the step
-  int32_t status;
 };
 
 // Last row whose prefix is <= i (0 <= i < prefix[rows]).
@@ -62,43 +57,51 @@ __device__ __forceinline__ int row_of(const int32_t *prefix, int rows, int i) {
     const int half = n >> 1;
     const bool right = prefix[lo + half] <= i;
     lo += right ? half : 0;
-    n -= half;
-    if (!right) n = half;
+    n = right ? n - half : half;
   }
   return lo;
 }
 
-// Scans the rows into s (LDS or global memory), checks the step, and writes
-// the state after it. All kScanThreads threads call it.
-__device__ StepTotals scan_step(const TablesParams &p, const StepRows &s) {
-  __shared__ int64_t s_sum[kScanThreads / 64][3];
-  __shared__ int s_flags[kScanThreads / 64];
+// Scans the rows into s and checks the step; `write`: also writes the state
+// after it. All NT threads of the workgroup call it.
+template <int NT>
+__device__ StepTotals scan_step(const TablesParams &p, const StepRows &s, bool write) {
+  __shared__ int64_t s_sum[NT / 64][3];
+  __shared__ int s_flags[NT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = (p.rows + kScanThreads - 1) / kScanThreads;
+  constexpr int kPer = (CLV_TABLES_MAX_ROWS + NT - 1) / NT;
+  const int per = (p.rows + NT - 1) / NT;
   const int b = min(p.rows, tid * per), e = min(p.rows, b + per);
   const int F = p.num_free[0];
-  auto row = [&](int r, int &len, int &held, int &n, int64_t &need) {
-    len = p.context_lens[r];
-    held = p.blocks_held[r];
-    n = p.new_lens[r];
-    need = held;
-    if (n > 0) {
-      const int64_t all = (int64_t)len + n + (held == 0 ? p.reserve : 0);
-      need = max((int64_t)held, (all + (1 << p.block_shift) - 1) >> p.block_shift);
+  // The thread's rows b .. e - 1 (past them: rows of nothing), read at once.
+  int len[kPer], held[kPer], n[kPer];
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    len[k] = held[k] = n[k] = 0;
+    if (b + k < e) {
+      len[k] = p.context_lens[b + k];
+      held[k] = p.blocks_held[b + k];
+      n[k] = p.new_lens[b + k];
     }
+  }
+  auto need = [&](int k) {  // blocks of row b + k after the step
+    const int64_t all = (int64_t)len[k] + n[k] + (held[k] == 0 ? p.reserve : 0);
+    const int64_t blocks = (all + (1 << p.block_shift) - 1) >> p.block_shift;
+    return n[k] > 0 ? max((int64_t)held[k], blocks) : (int64_t)held[k];
   };
   // Bit 0: a row longer than its table; bit 1: a state that cannot be.
   int64_t x[3] = {0, 0, 0};
   int flags = F < 0 || F > p.num_blocks ? 2 : 0;
-  for (int r = b; r < e; ++r) {
-    int len, held, n;
-    int64_t need;
-    row(r, len, held, n, need);
-    if (need > p.width) flags |= 1;
-    if (len < 0 || held < 0 || held > p.width || len > ((int64_t)held << p.block_shift)) flags |= 2;
-    x[0] += max(n, 0);
-    x[1] += need - held;
-    x[2] += n < 0 ? held : 0;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    if (b + k >= e) break;
+    if (need(k) > p.width) flags |= 1;
+    if (len[k] < 0 || held[k] < 0 || held[k] > p.width ||
+        len[k] > ((int64_t)held[k] << p.block_shift))
+      flags |= 2;
+    x[0] += max(n[k], 0);
+    x[1] += need(k) - held[k];
+    x[2] += n[k] < 0 ? held[k] : 0;
   }
   const int64_t own[3] = {x[0], x[1], x[2]};
 #pragma unroll
@@ -120,7 +123,8 @@ __device__ StepTotals scan_step(const TablesParams &p, const StepRows &s) {
 #pragma unroll
   for (int k = 0; k < 3; ++k) run[k] = x[k] - own[k];
   flags = 0;
-  for (int w = 0; w < kScanThreads / 64; ++w) {
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       if (w < wave) run[k] += s_sum[w][k];
@@ -128,125 +132,156 @@ __device__ StepTotals scan_step(const TablesParams &p, const StepRows &s) {
     }
     flags |= s_flags[w];
   }
+  int status = CLV_TABLES_OK;
+  if ((flags & 2) || F + all[2] > p.num_blocks) status = CLV_TABLES_BAD_STATE;
+  else if (all[1] > F + all[2]) status = CLV_TABLES_NO_BLOCKS;
+  else if (flags & 1) status = CLV_TABLES_ROW_FULL;
+  else if (all[0] > p.num_tokens) status = CLV_TABLES_NO_SLOTS;
+  const bool ok = status == CLV_TABLES_OK;
   StepTotals t;
-  if ((flags & 2) || F + all[2] > p.num_blocks) t.status = CLV_TABLES_BAD_STATE;
-  else if (all[1] > F + all[2]) t.status = CLV_TABLES_NO_BLOCKS;
-  else if (flags & 1) t.status = CLV_TABLES_ROW_FULL;
-  else if (all[0] > p.num_tokens) t.status = CLV_TABLES_NO_SLOTS;
-  else t.status = CLV_TABLES_OK;
-  const bool ok = t.status == CLV_TABLES_OK;
   t.num_free = F;
   t.tokens = ok ? (int32_t)all[0] : 0;
   t.take = ok ? (int32_t)all[1] : 0;
   t.gone = ok ? (int32_t)all[2] : 0;
   // In place, a row's state is read and written by the same thread, and every
   // thread has read the stack's count before the barrier above.
-  for (int r = b; r < e; ++r) {
-    int len, held, n;
-    int64_t need;
-    row(r, len, held, n, need);
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int r = b + k;
+    if (r >= e) break;
     s.tok[r] = ok ? (int32_t)run[0] : 0;
     s.take[r] = ok ? (int32_t)run[1] : 0;
     s.gone[r] = ok ? (int32_t)run[2] : 0;
-    s.len[r] = len;
-    s.held[r] = held;
-    p.query_start_loc[r] = ok ? (int32_t)run[0] : 0;
-    p.context_lens_out[r] = !ok ? len : n < 0 ? 0 : len + n;
-    p.blocks_held_out[r] = !ok ? held : n < 0 ? 0 : (int32_t)need;
-    run[0] += max(n, 0);
-    run[1] += need - held;
-    run[2] += n < 0 ? held : 0;
+    s.len[r] = len[k];
+    s.held[r] = held[k];
+    if (write) {
+      p.query_start_loc[r] = ok ? (int32_t)run[0] : 0;
+      p.context_lens_out[r] = !ok ? len[k] : n[k] < 0 ? 0 : len[k] + n[k];
+      p.blocks_held_out[r] = !ok ? held[k] : n[k] < 0 ? 0 : (int32_t)need(k);
+    }
+    run[0] += max(n[k], 0);
+    run[1] += need(k) - held[k];
+    run[2] += n[k] < 0 ? held[k] : 0;
   }
   if (tid == 0) {
     s.tok[p.rows] = t.tokens;
     s.take[p.rows] = t.take;
     s.gone[p.rows] = t.gone;
-    p.query_start_loc[p.rows] = t.tokens;
-    p.num_free_out[0] = F + t.gone - t.take;
-    p.status[0] = t.status;
+    if (write) {
+      p.query_start_loc[p.rows] = t.tokens;
+      p.num_free_out[0] = F + t.gone - t.take;
+      p.status[0] = status;
+    }
   }
+  __syncthreads();
   return t;
 }
 
-// Thread `at` of `n` serves its share of the step's pushed blocks, table
-// entries and slots.
-__device__ __forceinline__ void fill_step(const TablesParams &p, const StepRows &s,
-                                          const StepTotals &t, int64_t at, int64_t n) {
+// write: workgroup 0 writes the state; fill: the workgroups share the rest.
+template <int NT>
+__global__ void __launch_bounds__(NT) tables_step(const TablesParams p, bool write, bool fill) {
+  extern __shared__ int32_t s_rows[];
+  const StepRows s(s_rows, p.rows);
+  const StepTotals t = scan_step<NT>(p, s, write && blockIdx.x == 0);
+  if (!fill) return;
   const int F = t.num_free, R = t.gone, K = t.take;
-  // Block v of the stack V.
-  auto stack = [&](int v) {
-    if (v < F) return p.free_blocks[v];
+  // Where block v of the stack V stands.
+  auto stack = [&](int v) -> const int32_t * {
+    if (v < F) return p.free_blocks + v;
     const int r = row_of(s.gone, p.rows, v - F);
-    return p.block_tables[(int64_t)r * p.width + (v - F - s.gone[r])];
+    return p.block_tables + (int64_t)r * p.width + (v - F - s.gone[r]);
   };
-  for (int64_t i = at; i < R - K; i += n) p.free_blocks[F + i] = stack(F + (int)i);
-  for (int64_t i = at; i < K; i += n) {
-    const int r = row_of(s.take, p.rows, (int)i);
-    p.block_tables[(int64_t)r * p.width + s.held[r] + (i - s.take[r])] = stack(F + R - 1 - (int)i);
-  }
   const int mask = (1 << p.block_shift) - 1;
-  for (int64_t i = at; i < p.num_tokens; i += n) {
-    int64_t slot = -1;
-    if (i < t.tokens) {
-      const int r = row_of(s.tok, p.rows, (int)i);
-      const int pos = s.len[r] + ((int)i - s.tok[r]);
-      const int col = pos >> p.block_shift;
-      const int blk = col < s.held[r] ? p.block_tables[(int64_t)r * p.width + col]
-                                      : stack(F + R - 1 - (s.take[r] + col - s.held[r]));
-      slot = ((int64_t)blk << p.block_shift) + (pos & mask);
+  // One index space (slots in runs, taken blocks, pushed ones in runs), so that a
+  // thread's items do not wait for each other.
+  const int64_t runs = (p.num_tokens + kRun - 1) / kRun;
+  const int left = max(0, R - K);
+  const int64_t items = runs + K + (left + kRun - 1) / kRun;
+  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < items;
+       i += (int64_t)gridDim.x * NT) {
+    if (i >= runs + K) {
+      const int k0 = (int)(i - runs - K) * kRun;
+      int r = row_of(s.gone, p.rows, k0);
+      int32_t blk[kRun];
+#pragma unroll
+      for (int u = 0; u < kRun; ++u) {
+        const int k = min(k0 + u, left - 1);
+        while (s.gone[r + 1] <= k) ++r;
+        blk[u] = p.block_tables[(int64_t)r * p.width + (k - s.gone[r])];
+      }
+#pragma unroll
+      for (int u = 0; u < kRun; ++u)
+        if (k0 + u < left) p.free_blocks[F + k0 + u] = blk[u];
+    } else if (i >= runs) {
+      const int k = (int)(i - runs);
+      const int r = row_of(s.take, p.rows, k);
+      p.block_tables[(int64_t)r * p.width + s.held[r] + (k - s.take[r])] = *stack(F + R - 1 - k);
+    } else {
+      const int64_t i0 = i * kRun;
+      // The entries' places first, so that their loads are in flight together.
+      const int32_t *entry[kRun];
+      int pos[kRun];
+      int r = i0 < t.tokens ? row_of(s.tok, p.rows, (int)i0) : 0;
+#pragma unroll
+      for (int u = 0; u < kRun; ++u) {
+        entry[u] = p.num_free;
+        pos[u] = -1;
+        if (i0 + u < t.tokens) {
+          const int k = (int)i0 + u;
+          while (s.tok[r + 1] <= k) ++r;
+          pos[u] = s.len[r] + (k - s.tok[r]);
+          const int col = pos[u] >> p.block_shift;
+          if (u > 0 && col == (pos[u - 1] >> p.block_shift) && s.tok[r] < k)
+            entry[u] = entry[u - 1];  // the block of the token before it
+          else if (col < s.held[r])
+            entry[u] = p.block_tables + (int64_t)r * p.width + col;
+          else
+            entry[u] = stack(F + R - 1 - (s.take[r] + col - s.held[r]));
+        }
+      }
+      int64_t slot[kRun];
+#pragma unroll
+      for (int u = 0; u < kRun; ++u) slot[u] = *entry[u];
+#pragma unroll
+      for (int u = 0; u < kRun; ++u)
+        slot[u] = pos[u] < 0 ? -1 : (slot[u] << p.block_shift) + (pos[u] & mask);
+      typedef int64_t i64x2 __attribute__((ext_vector_type(2)));
+      int64_t *dst = p.slot_mapping + i0;
+      if (i0 + kRun <= p.num_tokens && ((uintptr_t)dst & 15u) == 0) {
+        store_vec<i64x2>(dst, (i64x2){slot[0], slot[1]});
+        store_vec<i64x2>(dst + 2, (i64x2){slot[2], slot[3]});
+      } else {
+#pragma unroll
+        for (int u = 0; u < kRun; ++u)
+          if (i0 + u < p.num_tokens) dst[u] = slot[u];
+      }
     }
-    p.slot_mapping[i] = slot;
   }
 }
 
-__global__ void __launch_bounds__(kScanThreads) tables_step(const TablesParams p) {
-  extern __shared__ int32_t s_rows[];
-  const StepRows s = step_rows(s_rows, p.rows);
-  const StepTotals t = scan_step(p, s);
-  __syncthreads();
-  fill_step(p, s, t, threadIdx.x, kScanThreads);
-}
-
-// The two launches of a larger step: the scan into the workspace (totals, then
-// the rows), and the rest of it over the chip.
-constexpr int kTotalsInts = 8;
-
-__global__ void __launch_bounds__(kScanThreads) tables_scan(const TablesParams p, int32_t *ws) {
-  const StepTotals t = scan_step(p, step_rows(ws + kTotalsInts, p.rows));
-  if (threadIdx.x == 0) *reinterpret_cast<StepTotals *>(ws) = t;
-}
-
-__global__ void __launch_bounds__(kFillThreads)
-tables_fill(const TablesParams p, const int32_t *__restrict__ ws) {
-  extern __shared__ int32_t s_rows[];
-  const StepTotals t = *reinterpret_cast<const StepTotals *>(ws);
-  const int n = 5 * p.rows + 3;
-  for (int i = threadIdx.x; i < n; i += kFillThreads) s_rows[i] = ws[kTotalsInts + i];
-  __syncthreads();
-  fill_step(p, step_rows(s_rows, p.rows), t, (int64_t)blockIdx.x * kFillThreads + threadIdx.x,
-            (int64_t)gridDim.x * kFillThreads);
-}
-
-size_t rows_bytes(int rows) { return (size_t)(5 * rows + 3) * 4; }
-
-// Steps that one workgroup serves.
-constexpr int64_t kSmallTokens = 8192;
+// In place, the state may only be written when every workgroup has read it:
+// up to this many tokens one workgroup serves the step, above it a second
+// launch writes the state.
+constexpr int64_t kInPlaceTokens = 8192;
 
 }  // namespace
 
-size_t tables_workspace_bytes(const TablesParams &p) {
-  return p.num_tokens <= kSmallTokens ? 0 : kTotalsInts * 4 + rows_bytes(p.rows);
-}
-
-hipError_t launch_tables(const TablesParams &p, void *workspace, hipStream_t stream) {
-  if (tables_workspace_bytes(p) == 0) {
-    hipLaunchKernelGGL(tables_step, dim3(1), dim3(kScanThreads), rows_bytes(p.rows), stream, p);
+hipError_t launch_tables(const TablesParams &p, hipStream_t stream) {
+  const bool in_place = p.blocks_held_out == p.blocks_held ||
+                        p.context_lens_out == p.context_lens || p.num_free_out == p.num_free;
+  const size_t lds = rows_bytes(p.rows);
+  if (in_place && p.num_tokens <= kInPlaceTokens) {
+    hipLaunchKernelGGL(tables_step<1024>, dim3(1), dim3(1024), lds, stream, p, true, true);
     return hipGetLastError();
   }
-  hipLaunchKernelGGL(tables_scan, dim3(1), dim3(kScanThreads), 0, stream, p, (int32_t *)workspace);
-  const int64_t groups = (p.num_tokens + 4 * kFillThreads - 1) / (4 * kFillThreads);
-  hipLaunchKernelGGL(tables_fill, dim3((unsigned)(groups < 1024 ? groups : 1024)),
-                     dim3(kFillThreads), rows_bytes(p.rows), stream, p, (const int32_t *)workspace);
+  // Workgroups for the slots, and two more for the blocks.
+  constexpr int NT = 256;
+  int64_t groups = p.num_tokens / (kRun * NT) + 3;
+  if (groups > 1024) groups = 1024;
+  hipLaunchKernelGGL(tables_step<NT>, dim3((unsigned)groups), dim3(NT), lds, stream, p, !in_place,
+                     true);
+  if (in_place)
+    hipLaunchKernelGGL(tables_step<NT>, dim3(1), dim3(NT), lds, stream, p, true, false);
   return hipGetLastError();
 }
 

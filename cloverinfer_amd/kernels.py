@@ -933,9 +933,5 @@ def advance_block_tables(block_tables: torch.Tensor, blocks_held: torch.Tensor,
                      blocks_held if blocks_held_out is None else blocks_held_out,
                      context_lens if context_lens_out is None else context_lens_out,
                      num_free if num_free_out is None else num_free_out)
-    dev = block_tables.device
-    lib = _native.load()
-    nbytes = lib.clv_tables_workspace_bytes(a)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _native.check(lib.clv_advance_block_tables(a, ws.data_ptr() if nbytes else None, nbytes,
-                                               _stream(dev)), "clv_advance_block_tables")
+    _native.check(_native.load().clv_advance_block_tables(a, _stream(block_tables.device)),
+                  "clv_advance_block_tables")

@@ -477,13 +477,8 @@ int clv_diff_prefill(const clv_prefill_args *args, const clv_diff_args *diff, vo
 
 size_t clv_diff_prefill_workspace_bytes(const clv_prefill_args *args);
 
-/* One step of the block tables (clv_tables_args). `workspace`: at least
- * clv_tables_workspace_bytes() bytes, 256-byte aligned; may be null where that
- * is 0. */
-int clv_advance_block_tables(const clv_tables_args *args, void *workspace,
-                             size_t workspace_bytes, clv_stream_t stream);
-
-size_t clv_tables_workspace_bytes(const clv_tables_args *args);
+/* One step of the block tables (clv_tables_args). Needs no workspace. */
+int clv_advance_block_tables(const clv_tables_args *args, clv_stream_t stream);
 
 #ifdef __cplusplus
 } /* extern "C" */
