@@ -277,17 +277,20 @@ _host_tried = False
 
 # What the native host code fills (host/call_args.cpp) and where: its
 # functions, and the layout they must have been compiled with.
-_FILLS = ("fill_decode_args", "fill_prefill_args", "fill_cache_args")
+_FILLS = ("fill_decode_args", "fill_prefill_args", "fill_cache_args", "fill_diff_args",
+          "fill_tables_args")
 
 
 def call_args_layout() -> tuple:
-    """ABI version, then size and the offsets of dtype and scale of each
-    argument block (the host module's ``call_args_layout``)."""
+    """ABI version, then size and the offsets of dtype and scale (of the block
+    tables' step num_tokens, of the differential block out_scale) of each argument block (the host module's
+    ``call_args_layout``)."""
     out = [ABI_VERSION]
     for cls in (DecodeArgs, PrefillArgs, CacheArgs):
         out += [ctypes.sizeof(cls), cls.dtype.offset]
         out += [cls.scale.offset] if cls is not CacheArgs else []
-    return tuple(out)
+    return (*out, ctypes.sizeof(TablesArgs), TablesArgs.num_tokens.offset,
+            ctypes.sizeof(DiffArgs), DiffArgs.out_scale.offset)
 
 
 def _checked_host(mod):

@@ -828,11 +828,11 @@ int fill_diff(const clv_diff_args *d, clv::DiffParams *out) {
   return CLV_OK;
 }
 
-// Least steps of a group of the balanced differential decode.
-#ifndef CLV_DIFF_MIN_STEPS
-#define CLV_DIFF_MIN_STEPS 4
-#endif
-constexpr int32_t kDiffMinSteps = CLV_DIFF_MIN_STEPS;
+// Least steps of a group of the balanced differential decode: fewer groups read
+// less each, more of them leave more partials to the merge. Four sequences of
+// 150..3900 tokens, 14/2 heads of 256, bf16: 1 step 25.5 us, 2 20.6, 4 19.5,
+// 8 22.7, 16 31.5; full batches have more steps a group than this anyway.
+constexpr int32_t kDiffMinSteps = 4;
 
 // `a` with the rows of both maps as its heads.
 int diff_rows(const clv_decode_args *a, clv_decode_args *rows) {
@@ -846,16 +846,36 @@ int diff_rows(const clv_decode_args *a, clv_decode_args *rows) {
 
 // Longest context for which a differential decode runs as one launch, a
 // workgroup per (sequence, kv head, 16 rows), where the caller names no wave
-// count (kernels.choose_schedule has the same bound for plain decode).
+// count (kernels.choose_schedule has the same bound for plain decode). One
+// launch / balanced, us, every sequence of the same length:
+//                                128        512        1024       2048
+//   8 seqs,   6/6 x 128  fp32    8.1/19.0   16.6/20.1  28.1/21.0  51.7/28.6
+//   8 seqs,  14/2 x 256  bf16    8.7/17.1   15.9/18.5  26.1/19.6  46.5/22.6
+//   64 seqs, 28/4 x 128  bf16    6.8/17.3   14.5/24.9  24.3/34.6  41.9/54.6
+//   128 seqs, 14/2 x 256 bf16    9.5/21.6   25.2/37.5  43.6/57.0  81.3/95.8
+// Past it one launch would still win for many sequences of one length, but it
+// takes as long as its longest sequence, which a ragged batch (what decodes
+// there) has alone.
 constexpr int32_t kDiffSinglePassMaxLen = 512;
+
+// Most segments (sequence x kv head x 16 rows) of head_dim 256 that take it. Two
+// workgroups of that width are resident on a compute unit (64.5 KiB of LDS for
+// the waves' join, as much for 2 rows as for 16), so more of them queue:
+// 16/16 x 256 fp16, 128 / 512 tokens: 512 segments 20.0/20.3 and 48.9/50.7 us,
+// 1024 38.8/29.6 and 93.3/91.5, 2048 74.1/53.4 and 183/171. head_dim 128 wins at
+// every count measured (1024 segments of 32/8 heads: 20.1/26.1 and 47.7/55.1).
+constexpr int64_t kDiffSinglePassWideSegments = 512;
 
 bool diff_single_pass(const clv_decode_args &rows, bool fp8, int32_t num_waves) {
   if (fp8) return false;
   if (!clv::diff_decode_mfma_supported(rows.head_dim, rows.block_size)) return true;
-  if (num_waves <= 0 && rows.max_context_len <= kDiffSinglePassMaxLen) return true;
+  const int64_t segments = (int64_t)rows.num_seqs * rows.num_kv_heads *
+                           ceil_div(rows.num_heads / rows.num_kv_heads, 16);
+  if (num_waves <= 0 && rows.max_context_len <= kDiffSinglePassMaxLen &&
+      (rows.head_dim <= 128 || segments <= kDiffSinglePassWideSegments))
+    return true;
   // More segments than the balanced decode takes: a workgroup each fills the chip.
-  return (int64_t)rows.num_seqs * rows.num_kv_heads *
-             ceil_div(rows.num_heads / rows.num_kv_heads, 16) > clv::kStreamMaxSegments;
+  return segments > clv::kStreamMaxSegments;
 }
 
 PrefillKernel diff_prefill_kernel(const clv::PrefillParams &p, DType dt) {
@@ -952,7 +972,7 @@ int clv_diff_prefill(const clv_prefill_args *a, const clv_diff_args *d, void *wo
   const clv::PrefillSplitShape sh = diff_split_shape(p, k);
   clv::PrefillSplit split;
   const clv::PrefillSplit *sp = nullptr;
-  if (sh.groups > 0) {
+  if (sh.groups > 0 && (workspace != nullptr || workspace_bytes != 0)) {
     if (workspace == nullptr || workspace_bytes < split_bytes(p, sh) ||
         ((uintptr_t)workspace & 255u) != 0)
       return CLV_EWORKSPACE;

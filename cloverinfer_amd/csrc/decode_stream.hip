@@ -748,11 +748,14 @@ hipError_t launch_sreduce_t(const DecodeParams &p, hipStream_t stream) {
   return launch_sreduce_tn<T, NEW, 1>(p, stream);
 }
 
-// Ring depth of the differential decode: as for plain decode at the same bytes
-// per step (16-bit pools three steps of up to 8 KiB a wave, two of 16 KiB).
+// Ring depth of the differential decode: three steps of loads in flight where a
+// key row has up to 256 bytes, one where it has more and a step's own loads are
+// enough. Depth 1/2/3, us, 128 sequences of 200..4096 tokens: 16-bit pools 4 kv
+// heads x 64 65.3/66.0/62.4, 4 x 128 99.1/99.9/98.3, 2 x 256 98.7/101.8/103.2;
+// fp32 6 x 128 249/251/254, 4 x 256 315/319/808 (3: registers spill).
 template <typename T, int D, bool KV8>
 hipError_t launch_diff_stream_td(const DecodeParams &p, hipStream_t stream) {
-  constexpr int DEPTH = D * (KV8 ? 1 : (int)sizeof(T)) > 256 ? 2 : 3;
+  constexpr int DEPTH = D * (KV8 ? 1 : (int)sizeof(T)) > 256 ? 1 : 3;
   const dim3 grid((unsigned)((p.num_waves + kWaves - 1) / kWaves));
   if (p.block_shift >= 4)
     hipLaunchKernelGGL((paged_decode_stream<T, D, true, DEPTH, false, KV8, false, true>), grid,

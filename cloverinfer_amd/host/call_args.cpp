@@ -57,7 +57,8 @@ bool dtypes_ok(const at::Tensor &x, const at::Tensor &k, bool *fp8) {
   return *fp8 || x.scalar_type() == k.scalar_type();
 }
 
-bool int_vector(const at::Tensor &t, at::ScalarType dt, int64_t n) {
+// A contiguous vector of n elements of type dt.
+bool is_vector(const at::Tensor &t, at::ScalarType dt, int64_t n) {
   return t.scalar_type() == dt && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
 }
 
@@ -110,7 +111,7 @@ bool fill_decode_args(uintptr_t dst, py::object out_, py::object q_, py::object 
   if (k->size(3) != q->size(2) || k->size(1) != block_size || k->size(2) == 0 ||
       q->size(1) % k->size(2) != 0 || !fits32(max_context_len))
     return false;
-  if (!int_matrix(*bt, q->size(0)) || !int_vector(*cl, at::kInt, q->size(0))) return false;
+  if (!int_matrix(*bt, q->size(0)) || !is_vector(*cl, at::kInt, q->size(0))) return false;
   a.out = out->data_ptr();
   a.q = q->data_ptr();
   a.k_cache = k->data_ptr();
@@ -153,8 +154,8 @@ bool fill_prefill_args(uintptr_t dst, py::object out_, py::object q_, py::object
       cl->dim() != 1 || !fits32(max_query_len))
     return false;
   const int64_t num_seqs = cl->size(0);
-  if (!fits32(num_seqs) || !int_matrix(*bt, num_seqs) || !int_vector(*cl, at::kInt, num_seqs) ||
-      !int_vector(*qsl, at::kInt, num_seqs + 1))
+  if (!fits32(num_seqs) || !int_matrix(*bt, num_seqs) || !is_vector(*cl, at::kInt, num_seqs) ||
+      !is_vector(*qsl, at::kInt, num_seqs + 1))
     return false;
   a.out = out->data_ptr();
   a.q = q->data_ptr();
@@ -195,7 +196,7 @@ bool fill_cache_args(uintptr_t dst, py::object key_, py::object value_, py::obje
       key->size(1) != k->size(2) || key->size(2) != k->size(3) || !fits32(key->size(0)) ||
       value->scalar_type() != key->scalar_type() || !dtypes_ok(*key, *k, &fp8) ||
       !dtype_code(key->scalar_type(), &a.dtype) || key->stride(2) != 1 || value->stride(2) != 1 ||
-      !int_vector(*slots, at::kLong, key->size(0)))
+      !is_vector(*slots, at::kLong, key->size(0)))
     return false;
   a.key = key->data_ptr();
   a.value = value->data_ptr();
@@ -218,11 +219,89 @@ bool fill_cache_args(uintptr_t dst, py::object key_, py::object value_, py::obje
   return true;
 }
 
+bool fill_diff_args(uintptr_t dst, py::object q_, py::object lam_, py::object weight_, double eps,
+                    double out_scale) {
+  const at::Tensor *q = plain(q_);
+  if (!q || q->dim() != 3) return false;
+  clv_diff_args a{};
+  if (THPVariable_Check(lam_.ptr())) {
+    const at::Tensor *lam = plain(lam_);
+    if (!lam || lam->scalar_type() != at::kFloat || !same_device(*q, *lam)) return false;
+    const int64_t dim = lam->dim();
+    if (dim < 1 || dim > 2 || lam->size(dim - 1) != q->size(1) ||
+        (dim == 2 && lam->size(0) != q->size(0)))
+      return false;
+    a.lambda = (const float *)lam->data_ptr();
+    a.lambda_stride_row = dim == 2 ? lam->stride(0) : 0;
+    a.lambda_stride_head = lam->stride(dim - 1);
+  } else {
+    if (!PyFloat_Check(lam_.ptr())) return false;
+    a.lambda_value = (float)PyFloat_AS_DOUBLE(lam_.ptr());
+  }
+  if (!weight_.is_none()) {
+    const at::Tensor *w = plain(weight_);
+    if (!w || !same_device(*q, *w) || !is_vector(*w, at::kFloat, q->size(2))) return false;
+    a.norm_weight = (const float *)w->data_ptr();
+  }
+  a.norm_eps = (float)eps;
+  a.out_scale = (float)out_scale;
+  *reinterpret_cast<clv_diff_args *>(dst) = a;
+  return true;
+}
+
+bool fill_tables_args(uintptr_t dst, py::object bt_, py::object held_, py::object cl_,
+                      py::object new_, py::object free_, py::object nfree_, int64_t block_size,
+                      py::object slots_, py::object qsl_, py::object status_, int64_t reserve,
+                      py::object held_out_, py::object cl_out_, py::object nfree_out_) {
+  const at::Tensor *bt = plain(bt_), *held = plain(held_), *cl = plain(cl_), *nw = plain(new_),
+                   *fr = plain(free_), *nfree = plain(nfree_), *slots = plain(slots_),
+                   *qsl = plain(qsl_), *status = plain(status_), *held_out = plain(held_out_),
+                   *cl_out = plain(cl_out_), *nfree_out = plain(nfree_out_);
+  if (!bt || !held || !cl || !nw || !fr || !nfree || !slots || !qsl || !status || !held_out ||
+      !cl_out || !nfree_out ||
+      !same_device(*bt, *held, *cl, *nw, *fr, *nfree, *slots, *qsl, *status, *held_out, *cl_out,
+                   *nfree_out))
+    return false;
+  if (bt->dim() != 2 || fr->dim() != 1 || slots->dim() != 1) return false;
+  const int64_t rows = bt->size(0);
+  if (!fits32(rows) || !int_matrix(*bt, rows) || !fits32(fr->size(0)) || !fits32(block_size) ||
+      !fits32(reserve) || !is_vector(*held, at::kInt, rows) || !is_vector(*cl, at::kInt, rows) ||
+      !is_vector(*nw, at::kInt, rows) || !is_vector(*fr, at::kInt, fr->size(0)) ||
+      !is_vector(*nfree, at::kInt, 1) || !is_vector(*qsl, at::kInt, rows + 1) ||
+      !is_vector(*status, at::kInt, 1) || !is_vector(*held_out, at::kInt, rows) ||
+      !is_vector(*cl_out, at::kInt, rows) || !is_vector(*nfree_out, at::kInt, 1) ||
+      !is_vector(*slots, at::kLong, slots->size(0)))
+    return false;
+  clv_tables_args a{};
+  a.block_tables = (int32_t *)bt->data_ptr();
+  a.blocks_held = (const int32_t *)held->data_ptr();
+  a.context_lens = (const int32_t *)cl->data_ptr();
+  a.new_lens = (const int32_t *)nw->data_ptr();
+  a.free_blocks = (int32_t *)fr->data_ptr();
+  a.num_free = (const int32_t *)nfree->data_ptr();
+  a.blocks_held_out = (int32_t *)held_out->data_ptr();
+  a.context_lens_out = (int32_t *)cl_out->data_ptr();
+  a.num_free_out = (int32_t *)nfree_out->data_ptr();
+  a.slot_mapping = (int64_t *)slots->data_ptr();
+  a.query_start_loc = (int32_t *)qsl->data_ptr();
+  a.status = (int32_t *)status->data_ptr();
+  a.num_tokens = slots->size(0);
+  a.rows = (int32_t)rows;
+  a.width = (int32_t)bt->size(1);
+  a.block_size = (int32_t)block_size;
+  a.num_blocks = (int32_t)fr->size(0);
+  a.reserve = (int32_t)reserve;
+  *reinterpret_cast<clv_tables_args *>(dst) = a;
+  return true;
+}
+
 py::tuple call_args_layout() {
   return py::make_tuple(
       (size_t)CLV_ABI_VERSION, sizeof(clv_decode_args), offsetof(clv_decode_args, dtype),
       offsetof(clv_decode_args, scale), sizeof(clv_prefill_args), offsetof(clv_prefill_args, dtype),
-      offsetof(clv_prefill_args, scale), sizeof(clv_cache_args), offsetof(clv_cache_args, dtype));
+      offsetof(clv_prefill_args, scale), sizeof(clv_cache_args), offsetof(clv_cache_args, dtype),
+      sizeof(clv_tables_args), offsetof(clv_tables_args, num_tokens), sizeof(clv_diff_args),
+      offsetof(clv_diff_args, out_scale));
 }
 
 }  // namespace clv_host

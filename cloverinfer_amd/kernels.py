@@ -8,6 +8,7 @@ call goes through ``libclover_attn.so``; tensors must live on a HIP device.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import math
@@ -86,6 +87,18 @@ def _stream(dev: torch.device) -> int:
     if _raw_stream is not None and dev.index is not None:
         return _raw_stream(dev.index)
     return torch.cuda.current_stream(dev).cuda_stream
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_here = contextlib.nullcontext()
+
+
+def _on(dev: torch.device):
+    """A context in which ``dev`` is the current device: the default stream's
+    handle and the library's device queries mean the current one's."""
+    if dev.type != "cuda" or dev.index is None or dev.index == _current_device():
+        return _here
+    return torch.cuda.device(dev)
 
 
 def _filled(name: str, args, *values):
@@ -749,8 +762,12 @@ def chunked_prefill(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
         _native.check(lib.clv_chunked_prefill(a, _stream(dev)), "clv_chunked_prefill")
 
 
-def _diff_args(lam, norm_weight, norm_eps, out_scale, rows, num_heads, head_dim,
-               dev) -> _native.DiffArgs:
+def _diff_args(q, lam, norm_weight, norm_eps, out_scale) -> _native.DiffArgs:
+    a = _filled("fill_diff_args", _native.DiffArgs(), q, lam, norm_weight, norm_eps, out_scale)
+    if a is not None:
+        return a
+    rows, num_heads, head_dim = q.shape
+    dev = q.device
     a = _native.DiffArgs()
     if isinstance(lam, torch.Tensor):
         if lam.device != dev:
@@ -808,21 +825,21 @@ def differential_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Te
     a = _decode_args(out, q, k_cache, v_cache, block_tables, context_lens, block_size,
                      max_context_len, _half_scale(scale, q))
     dev = q.device
-    d = _diff_args(lam, norm_weight, norm_eps, out_scale, a.num_seqs, a.num_heads, a.head_dim, dev)
+    d = _diff_args(q, lam, norm_weight, norm_eps, out_scale)
     lib = _native.load()
-    stream = _stream(dev)
     fp8 = k_cache.dtype == FP8
     ks = vs = None
-    if fp8:
-        ks = kv_scales(k_scale, a.num_kv_heads, dev)
-        vs = kv_scales(v_scale, a.num_kv_heads, dev)
-    nbytes = lib.clv_diff_decode_workspace_bytes(a, fp8, num_waves)
-    # From the caching allocator, as in chunked_prefill.
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _native.check(lib.clv_diff_decode(a, d, ks.data_ptr() if fp8 else None,
-                                      vs.data_ptr() if fp8 else None, num_waves,
-                                      ws.data_ptr() if nbytes else None, nbytes, stream),
-                  "clv_diff_decode")
+    with _on(dev):
+        if fp8:
+            ks = kv_scales(k_scale, a.num_kv_heads, dev)
+            vs = kv_scales(v_scale, a.num_kv_heads, dev)
+        nbytes = lib.clv_diff_decode_workspace_bytes(a, fp8, num_waves)
+        # From the caching allocator, as in chunked_prefill.
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        _native.check(lib.clv_diff_decode(a, d, ks.data_ptr() if fp8 else None,
+                                          vs.data_ptr() if fp8 else None, num_waves,
+                                          ws.data_ptr() if nbytes else None, nbytes,
+                                          _stream(dev)), "clv_diff_decode")
 
 
 def differential_prefill(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor,
@@ -845,12 +862,19 @@ def differential_prefill(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tens
         a = _prefill_args(out, q, k_cache, v_cache, block_tables, context_lens, query_start_loc,
                           max_query_len, scale)
     dev = q.device
-    d = _diff_args(lam, norm_weight, norm_eps, out_scale, a.num_tokens, a.num_heads, a.head_dim, dev)
+    d = _diff_args(q, lam, norm_weight, norm_eps, out_scale)
     lib = _native.load()
-    nbytes = lib.clv_diff_prefill_workspace_bytes(a)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _native.check(lib.clv_diff_prefill(a, d, ws.data_ptr() if nbytes else None, nbytes,
-                                       _stream(dev)), "clv_diff_prefill")
+    with _on(dev):
+        nbytes = lib.clv_diff_prefill_workspace_bytes(a)
+        ws = None
+        if nbytes:
+            # As in chunked_prefill, with the form that needs none behind it.
+            try:
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            except torch.cuda.OutOfMemoryError:
+                nbytes = 0
+        _native.check(lib.clv_diff_prefill(a, d, ws.data_ptr() if nbytes else None, nbytes,
+                                           _stream(dev)), "clv_diff_prefill")
 
 
 # advance_block_tables' status (the value it leaves in ``status``).
@@ -860,6 +884,11 @@ TABLES_OK, TABLES_NO_BLOCKS, TABLES_ROW_FULL, TABLES_NO_SLOTS, TABLES_BAD_STATE 
 def _tables_args(block_tables, blocks_held, context_lens, new_lens, free_blocks, num_free,
                  block_size, slot_mapping, query_start_loc, status, reserve, blocks_held_out,
                  context_lens_out, num_free_out) -> _native.TablesArgs:
+    a = _filled("fill_tables_args", _native.TablesArgs(), block_tables, blocks_held, context_lens,
+                new_lens, free_blocks, num_free, block_size, slot_mapping, query_start_loc, status,
+                reserve, blocks_held_out, context_lens_out, num_free_out)
+    if a is not None:
+        return a
     _require_device(block_tables, blocks_held, context_lens, new_lens, free_blocks, num_free,
                     slot_mapping, query_start_loc, status, blocks_held_out, context_lens_out,
                     num_free_out)
@@ -933,5 +962,7 @@ def advance_block_tables(block_tables: torch.Tensor, blocks_held: torch.Tensor,
                      blocks_held if blocks_held_out is None else blocks_held_out,
                      context_lens if context_lens_out is None else context_lens_out,
                      num_free if num_free_out is None else num_free_out)
-    _native.check(_native.load().clv_advance_block_tables(a, _stream(block_tables.device)),
-                  "clv_advance_block_tables")
+    dev = block_tables.device
+    with _on(dev):
+        _native.check(_native.load().clv_advance_block_tables(a, _stream(dev)),
+                      "clv_advance_block_tables")

@@ -469,8 +469,8 @@ size_t clv_diff_decode_workspace_bytes(const clv_decode_args *args, int32_t fp8,
 /*
  * Differential attention of each sequence's new rows over its paged context:
  * clv_chunked_prefill's call with the two maps of clv_diff_args. `workspace` as
- * above, sized by clv_diff_prefill_workspace_bytes(). No counterpart in the
- * reference.
+ * above, sized by clv_diff_prefill_workspace_bytes(); NULL with 0 bytes runs the
+ * form that needs none. No counterpart in the reference.
  */
 int clv_diff_prefill(const clv_prefill_args *args, const clv_diff_args *diff, void *workspace,
                      size_t workspace_bytes, clv_stream_t stream);

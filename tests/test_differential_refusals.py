@@ -2,6 +2,7 @@
 on CPU tensors (with the device check alone taken out) and through the C ABI
 without a GPU; and the float64 restatements on their own."""
 import ctypes
+import types
 
 import pytest
 import torch
@@ -265,3 +266,52 @@ def test_restated_rows_by_hand():
     assert torch.allclose(r["out"][0, 0], want)
     n = od.rows(q, k, v, [2], 0.5, torch.full((4,), 2.0), eps=0.0, out_scale=0.3, scale=1.0)
     assert torch.allclose(n["out"][0, 0], 0.3 * 2.0 * want / want.square().mean().sqrt())
+
+
+@pytest.mark.parametrize("room", [True, False])
+def test_prefill_without_room_for_a_workspace(monkeypatch, room):
+    """On a full device the call runs as the form that needs no memory."""
+    t = decode_tensors()
+    calls = []
+    lib = types.SimpleNamespace(
+        clv_diff_prefill_workspace_bytes=lambda a: 4096,
+        clv_diff_prefill=lambda a, d, ws, n, s: calls.append((ws is not None, n)) or 0)
+
+    def empty(*size, **kw):
+        if not room:
+            raise torch.cuda.OutOfMemoryError("no room")
+        return torch.zeros(*size, **kw)
+
+    monkeypatch.setattr(kernels, "_require_device", lambda *t: t[0].device)
+    monkeypatch.setattr(kernels._native, "load", lambda: lib)
+    monkeypatch.setattr(kernels, "_stream", lambda dev: 0)
+    monkeypatch.setattr(torch, "empty", empty)
+    kernels.differential_prefill(*t, torch.arange(4, dtype=torch.int32), 1, 0.5)
+    assert calls == [(True, 4096) if room else (False, 0)]
+
+
+def test_launches_run_with_their_tensors_device_current(monkeypatch):
+    """On tensors of another device than the current one the call changes to
+    it: the default stream and the device queries are the current device's."""
+    here, trace = [0], []
+
+    class Guard:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            trace.append(self.dev.index)
+            here[0] = self.dev.index
+
+        def __exit__(self, *exc):
+            here[0] = 0
+
+    monkeypatch.setattr(kernels, "_current_device", lambda: here[0])
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    for index in (0, 1):
+        with kernels._on(torch.device("cuda", index)):
+            assert here[0] == index
+        assert here[0] == 0
+    with kernels._on(torch.device("cpu")):
+        pass
+    assert trace == [1]

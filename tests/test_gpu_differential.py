@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from cloverinfer_amd import kernels
+from cloverinfer_amd import _native, kernels
 from oracle import differential as od
 from tests.helpers import make_paged_kv, padded_tables
 
@@ -476,3 +476,55 @@ def test_repeated_calls_are_bit_equal_and_streams_do_not_share():
     torch.cuda.synchronize()
     for w, outs in zip(want, got):
         assert all(torch.equal(w, o) for o in outs)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype,cached,new", [
+    (6, 6, 128, torch.float32, [100, 0], [200, 30]),
+    (6, 2, 128, torch.bfloat16, [50, 300], [1000, 40]),
+    (3, 1, 256, torch.float16, [0, 300], [1030, 7]),
+])
+def test_prefill_without_a_workspace(monkeypatch, hq, hkv, d, dtype, cached, new):
+    """Where the device has no room for a split prefill's partials, the form
+    that needs none answers."""
+    real, refused = torch.empty, []
+
+    def empty(*size, **kw):
+        if kw.get("dtype") is torch.uint8:
+            refused.append(size[0])
+            raise torch.cuda.OutOfMemoryError("no room")
+        return real(*size, **kw)
+
+    split = _prefill(cached, new, hq, hkv, d, dtype)
+    monkeypatch.setattr(torch, "empty", empty)
+    whole = _prefill(cached, new, hq, hkv, d, dtype)
+    monkeypatch.undo()
+    assert len(refused) == 1 and refused[0] > 0
+    assert whole.shape == split.shape
+
+
+def test_decode_many_short_wide_rows():
+    """head_dim 256 past the segments that one launch takes."""
+    _decode([(i * 7) % 40 for i in range(130)], 4, 4, 256, torch.float16)
+
+
+def test_native_argument_block_is_the_python_one(monkeypatch):
+    """The native host code fills the block that the Python checks fill, and
+    leaves what they refuse, or take in another form, to them."""
+    q = torch.zeros(3, 8, 64, dtype=torch.float16, device=DEV)
+    lam = torch.rand(3, 8, device=DEV)
+    weight = torch.rand(64, device=DEV)
+    real = kernels._filled
+    for x in (0.25, lam, lam[0], torch.rand(8, 3, device=DEV).t(), torch.rand(16, device=DEV)[::2]):
+        for w in (None, weight):
+            assert real("fill_diff_args", _native.DiffArgs(), q, x, w, 1e-6, 0.2) is not None
+            native = bytes(kernels._diff_args(q, x, w, 1e-6, 0.2))
+            monkeypatch.setattr(kernels, "_filled", lambda *a: None)
+            assert bytes(kernels._diff_args(q, x, w, 1e-6, 0.2)) == native
+            monkeypatch.setattr(kernels, "_filled", real)
+    assert kernels._diff_args(q, 1, None, 1e-6, 0.2).lambda_value == 1.0
+    for x, w in ((lam.double(), None), (lam[:2], None), (lam[:, :7], None), (lam.cpu(), None),
+                 (lam[None], None), (0.2, weight.half()), (0.2, weight[:32]), (0.2, weight.cpu()),
+                 (0.2, torch.rand(128, device=DEV)[::2]), (lam[0, 0], None)):
+        assert real("fill_diff_args", _native.DiffArgs(), q, x, w, 1e-6, 0.2) is None
+        with pytest.raises(ValueError):
+            kernels._diff_args(q, x, w, 1e-6, 0.2)

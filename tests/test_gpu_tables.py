@@ -7,7 +7,7 @@ import random
 import pytest
 import torch
 
-from cloverinfer_amd import kernels
+from cloverinfer_amd import _native, kernels
 from oracle import differential as od
 
 pytestmark = pytest.mark.gpu
@@ -174,3 +174,28 @@ def test_graph_replays_advance_the_state(tokens):
         assert st.dev[0].tolist() == st.table and qsl.tolist() == want_qsl
         if i % 5 == 2:
             st.step([0, 0, 1, 0, 0, 0], 9000)
+
+
+def test_native_argument_block_is_the_python_one(monkeypatch):
+    """The native host code fills the block that the Python checks fill, in
+    place and out of place, and leaves what they refuse to them."""
+    n = 5
+    t = [_i32([[-1] * 3] * n), _i32([0] * n), _i32([0] * n), _i32([1] * n), _i32(list(range(9))),
+         _i32([9]), 16, torch.zeros(n, dtype=torch.int64, device=DEV), _i32([0] * (n + 1)),
+         _i32([0]), 1]
+    outs = [torch.empty_like(t[1]), torch.empty_like(t[2]), torch.empty_like(t[5])]
+    real = kernels._filled
+    for o in (outs, [t[1], t[2], t[5]]):
+        assert real("fill_tables_args", _native.TablesArgs(), *t, *o) is not None
+        native = bytes(kernels._tables_args(*t, *o))
+        monkeypatch.setattr(kernels, "_filled", lambda *a: None)
+        assert bytes(kernels._tables_args(*t, *o)) == native
+        monkeypatch.setattr(kernels, "_filled", real)
+    wrong = {0: t[0].long(), 1: t[1][:4], 2: t[2].cpu(), 3: t[3][::2], 4: t[4][None], 5: _i32([1, 2]),
+             7: t[7].int(), 8: t[8][1:], 9: t[9][:0]}
+    for i, w in wrong.items():
+        bad = list(t)
+        bad[i] = w
+        assert real("fill_tables_args", _native.TablesArgs(), *bad, *outs) is None, i
+        with pytest.raises((ValueError, RuntimeError)):
+            kernels._tables_args(*bad, *outs)
