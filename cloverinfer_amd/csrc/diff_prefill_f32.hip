@@ -1,16 +1,25 @@
 // diff_prefill_f32.hip - differential attention of chunked prefill with fp32
 // MFMAs (fp32 operands and accumulation throughout), over paged KV.
 //
-// A workgroup (4 waves, two workgroups per CU) takes kPairs = 32 rows = bq
+// A workgroup (4 waves, two or three workgroups per CU) takes kPairs = 32 rows = bq
 // tokens x G query heads of one kv head: waves w and w + 2 hold the same 16
 // rows, one map each, and meet through LDS at the end. Tiles of K and V go
 // through a two-stage LDS ring, the global loads of tile k + 1 in flight while
 // tile k is computed; items are split evenly over the workgroups
-// (prefill_split.h). Fragments, the order of the sums and their trees are those
-// of the plain fp32 prefill, over the map's half of every key row: score MFMA
-// (i, e) takes d = 16i + 4j + e of the half, o[4w + e] holds columns 64w + 4 n16
-// + e, a score is a tree over chains of two MFMAs, and P.V of a tile joins the
-// running accumulator once per tile.
+// (prefill_split.h). Fragments are those of the plain fp32 prefill, over the
+// map's half of every key row: score MFMA (i, e) takes d = 16i + 4j + e of the
+// half, o[4w + e] holds columns 64w + 4 n16 + e.
+//
+// Bound by the matrix core and by the vector instructions beside it, which add
+// to its time rather than hide in it: a score is two chains of MFMAs and P.V of
+// a tile one chain per column block, which joins the running accumulator once
+// per tile (a sum over n tokens has n / 16 roundings in a row at most). Trees over
+// chains of two, as in the plain form, cost 100 additions a tile more: 8 prompts
+// of 2048 tokens, 6/6 heads of 128, 913 us against 844, 16/4 of 256 2437 and 2122.
+// 8 x 1024 tokens of 6/6 heads run 215 us (90 TFLOP/s). Short prompts (17..512
+// tokens, 50 us) are bound by what a workgroup waits for before its first tile
+// and between items: schedule 2, cursor 3, Q and the first tile 2, an item's
+// end 2..4 us, then 2.9 us per tile of 16 tokens with three workgroups per CU.
 #include "prefill_split.h"
 
 namespace clv {
@@ -19,22 +28,29 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kPairs = kWaves / 2 * 16;  // rows per workgroup
-constexpr int kPerCu = 2;                // workgroups per CU: LDS at head_dim 128 and 256
 
-// Tokens per tile: 16 at head_dim 256, where a token's rows take twice the LDS.
-template <int D> constexpr int tile_tokens() { return D == 256 ? 16 : 32; }
+// Tokens per tile and workgroups per CU. At head_dim 128 tiles of 16 leave LDS
+// and registers for three workgroups, against two with tiles of 32: 8 x 1024
+// tokens 215 and 245 us, 17..512 tokens 52.6 and 52.1. At 64 three fit with 32
+// (4 x 1024 tokens of 16/4 heads 166 us, two 177); 256 needs the registers of two.
+template <int D> constexpr int tile_tokens() { return D == 64 ? 32 : 16; }
+template <int D> constexpr int per_cu() { return D == 256 ? 2 : 3; }
 
 template <int D> struct SplitCfg {
   static constexpr int kBK = tile_tokens<D>();
+  // Items at 1/2/3/4 units, 23 batches of all head dims, sum: 2443, 2466, 2492,
+  // 2532 us. kMinShare, kCutUnits at 48, 64, 96 and 128 tokens: equal within 0.5 %.
   static constexpr int kItemUnits = 1;
-  static constexpr int kMinShare = 3;
-  static constexpr int kCutUnits = 3;
+  static constexpr int kMinShare = 96 / kBK;
+  static constexpr int kCutUnits = 96 / kBK;
   static __host__ __device__ __forceinline__ int tile_units(int) { return 1; }
   static __host__ __device__ __forceinline__ int snap(int share) { return max(1, share / 16); }
 };
 
-// Table width in tokens up to which a call is not split.
-constexpr int kSplitMinTokens = 192;
+// Table width in tokens up to which a call is not split: 8 x 256 tokens of 6/6
+// heads of 128 40.5 us unsplit and 43.3 split, 4 of 16/4 of 64 25.0 and 30.0
+// (of 256 75.3 and 73.0); 8 x 512 of 6/6 94 and 82.
+constexpr int kSplitMinTokens = 256;
 
 __device__ __forceinline__ f32x4 mfma(uint32_t a, uint32_t b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, a),
@@ -69,12 +85,11 @@ __device__ __forceinline__ float seen_v(const int *seen_by, int col, int last) {
 }
 
 template <int D, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, kPerCu)
+__global__ void __launch_bounds__(kThreads, per_cu<D>())
 diff_prefill_f32(const PrefillArgs args) {
   constexpr int kBK = tile_tokens<D>();
   constexpr int H = kBK / 16;            // 16-token steps per tile
   constexpr int NQK = D / 32;            // 16-byte Q / K words per lane of a half head
-  constexpr int NCH = NQK < 4 ? NQK : 4; // words per tree of the score
   constexpr int CH = D / 16;             // output blocks
   constexpr int ROW = D + 4;             // LDS row stride (floats)
   constexpr int CPR = D / 4;             // 16-byte chunks per row
@@ -250,26 +265,18 @@ diff_prefill_f32(const PrefillArgs args) {
       if (tile < te_w) {
         const float *K = sK + buf * kStage + map * (D / 2);
         const float *V = sV + buf * kStage;
-        // Scores: chains of two MFMAs (eight products), joined by a tree.
+        // Scores: two chains of MFMAs.
         f32x4 sacc[H];
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-          f32x4 part[NQK / NCH];
+          f32x4 ch[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-          for (int i4 = 0; i4 < NQK; i4 += NCH) {
-            f32x4 ch[8];
+          for (int i = 0; i < NQK; ++i) {
+            const u32x4 k = load_vec<u32x4>(&K[(16 * h + n16) * ROW + 16 * i + 4 * j]);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) ch[u] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < NCH; ++i) {
-              const u32x4 k = load_vec<u32x4>(&K[(16 * h + n16) * ROW + 16 * (i4 + i) + 4 * j]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                ch[4 * (i & 1) + e] = mfma(k[e], q[i4 + i][e], ch[4 * (i & 1) + e]);
-            }
-            part[i4 / NCH] = ((ch[0] + ch[1]) + (ch[2] + ch[3])) + ((ch[4] + ch[5]) + (ch[6] + ch[7]));
+            for (int e = 0; e < 4; ++e) ch[e & 1] = mfma(k[e], q[i][e], ch[e & 1]);
           }
-          sacc[h] = NQK / NCH == 2 ? part[0] + part[NQK / NCH - 1] : part[0];
+          sacc[h] = ch[0] + ch[1];
         }
         const bool full = __all(sValid[buf][lane % kBK] != 0) && tile * kBK + kBK - 1 <= lim_first;
         // Scores a row may not see become -inf.
@@ -317,18 +324,12 @@ diff_prefill_f32(const PrefillArgs args) {
               v[h][k] = load_vec<u32x4>(&V[(16 * h + 4 * j + k) * ROW + 64 * w + 4 * n16]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            f32x4 t[H][2];
-#pragma unroll
-            for (int h = 0; h < H; ++h)
-#pragma unroll
-              for (int k = 0; k < 2; ++k) t[h][k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+            f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
               for (int h = 0; h < H; ++h)
-                t[h][k & 1] = mfma(__builtin_bit_cast(uint32_t, pr[h][k]), v[h][k][e], t[h][k & 1]);
-            f32x4 sum = t[0][0] + t[0][1];
-            if constexpr (H == 2) sum = sum + (t[H - 1][0] + t[H - 1][1]);
+                sum = mfma(__builtin_bit_cast(uint32_t, pr[h][k]), v[h][k][e], sum);
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               o[4 * w + e][r] = __builtin_fmaf(o[4 * w + e][r], ar[r], sum[r]);
@@ -463,8 +464,9 @@ bool diff_prefill_f32_covers(const PrefillParams &p) {
 }
 
 PrefillSplitShape diff_prefill_f32_split_shape(const PrefillParams &p) {
-  const int bk = p.head_dim == 256 ? tile_tokens<256>() : tile_tokens<128>();
-  return prefill_split_shape(p, kPairs, bk, kPerCu, 1, kSplitMinTokens / bk, false);
+  const int bk = p.head_dim == 64 ? tile_tokens<64>() : tile_tokens<128>();
+  const int per = p.head_dim == 256 ? per_cu<256>() : per_cu<128>();
+  return prefill_split_shape(p, kPairs, bk, per, 1, kSplitMinTokens / bk, false);
 }
 
 hipError_t launch_diff_prefill_f32(const PrefillParams &p, const PrefillSplit *sp,
