@@ -9,7 +9,8 @@
 // 64 kRT rows (row r is token r / G, query head r % G of one kv head) against
 // all K/V tiles its last row sees, staged in LDS. Waves w and w + 4 hold the
 // same 16 kRT rows, one map each: a wave reads only its half of every key row
-// (D/64 k-steps of 32), and the pair meets once, at the end, through LDS. Per 32
+// (D/64 k-steps of 32), and the pair meets once, at the end, through LDS, where
+// each wave finishes half of the rows. Per 32
 // tokens a wave runs
 //   S^T[t, r] = K_m[t, :] . Q_m[r, :]   2 x kRT x D/64 MFMAs (16x16x32)
 //   O[r, d]  += P[r, t] V[t, d]         kRT x D/16 MFMAs
@@ -27,6 +28,17 @@
 // pass that keeps bf16 V as it is and P as a bf16 value and its residual, with 0
 // in the place of infinities and NaN, which only the rows that see them then take
 // (0 * inf is NaN). The running maximum is only raised by more than 2^8.
+//
+// What bounds it. At head_dim 128: the matrix core with the vector work beside
+// it, which adds to its time (16x16x32 products 265 us of the 541 of eight chunks
+// of 512 over 4096 tokens, 32/8 heads, bf16; staging, conversion and softmax the
+// rest): 810 TFLOP/s. Products of 32x32x16 (558 us), exponentials between the
+// products of one wave (584), scores a step ahead (564) and a barrier between
+// the waves' phases (553) were no faster; nor were two to eight V operands in
+// flight (526..541). At head_dim 256: LDS reads, 24 KiB a wave and 32 tokens for
+// 25 products: 320 us for four chunks of 512 over 4096 tokens, 16/4 heads (600
+// TFLOP/s). Two row tiles a wave would halve them but spill, and cost small
+// calls their rows: 287 us there, 34 -> 53 for a prompt of 777 tokens.
 #include "prefill_split.h"
 
 #include <type_traits>
@@ -65,19 +77,27 @@ __device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
 }
 
-// Units of the split (prefill_split.h): a quarter of the time of a full tile.
+// Units of the split (prefill_split.h): tiles, full or not (D = 256: 1.26 us with all
+// rows, 1.13 with 7 of 64). An item costs what its start (Q, first tile) and end
+// (join, or partials and their merge) take, 8..10 us: four tiles of 64 tokens, six
+// of 32. Sum over 46 batches (chunks, prompts, mixed steps; head_dim 64, 128, 256):
+// items at two tiles, a bound moved by up to 1/16 of a share 4860 us, as below,
+// 1/64 4638; the least share six tiles in place of four and a cut five in place of
+// ten 4600 (cut 16: 4612, 25: 4624; least share eight: 4638, twelve 4642).
 template <int D> struct SplitCfg {
   static constexpr int kBK = Shape<D>::kBK;
-  static constexpr int kItemUnits = 8;
-  static constexpr int kMinShare = 16;
-  static constexpr int kCutUnits = 40;
-  static __host__ __device__ __forceinline__ int tile_units(int rows) {
-    return rows > Shape<D>::kPairs / 2 ? 4 : 3;
+  static constexpr int kItemUnits = D == 256 ? 6 : 4;
+  static constexpr int kMinShare = 6;
+  static constexpr int kCutUnits = 5;
+  static __host__ __device__ __forceinline__ int tile_units(int) { return 1; }
+  static __host__ __device__ __forceinline__ int snap(int share) {
+    return max(kItemUnits, share / 64);
   }
-  static __host__ __device__ __forceinline__ int snap(int share) { return max(8, share / 16); }
 };
 
-// Table width in tokens up to which a call is not split.
+// Table width in tokens up to which a call is not split (91 batches of 1..1024
+// tokens, sum: 128 3701 us, 256 3665, 512 3451, 1024 3322; 91 of up to 5000 tokens:
+// 1024 7291, 1536 7425, 2048 8087, 4096 10130).
 constexpr int kSplitMinTokens = 1024;
 
 // Eight values of V (token `pos`, columns d0 ..) with 0 in the place of NaN and
@@ -132,7 +152,7 @@ diff_prefill_mfma(const PrefillArgs args) {
   constexpr int PASSES = kBK / RPP;       // load passes per tile
   constexpr int kStage = kBK * KROW;      // elements of a stage of K (and of V)
   constexpr int kLdsK = 3 * kStage * 2, kLdsAll = 2 * kLdsK;
-  constexpr int kLdsPair = kWaves / 2 * kRT * CH * 64 * 16;  // the second maps' rows
+  constexpr int kLdsPair = kWaves * kRT * CH * 64 * 8;  // half of every wave's rows
   static_assert(kLdsPair <= kLdsAll, "the pairs meet in the tile ring's memory");
 
   __shared__ __attribute__((aligned(16))) char s_mem[kLdsAll];
@@ -550,46 +570,56 @@ diff_prefill_mfma(const PrefillArgs args) {
   const PrefillArgs ar1 = SPLIT ? reload_args() : args;
   const bool whole = !SPLIT || (t0 == 0 && t1 == nt);
   if (whole) {
-    // The second map's rows go to the first map's wave in its own layout.
-    f32x4 *meet = (f32x4 *)s_mem + (size_t)(wave % (kWaves / 2)) * kRT * CH * 64 + lane;
-    if (map == 1 && active) {
+    // The two waves of a pair finish half of its rows each: those of the
+    // accumulators' elements 0 and 1 the first map's wave, 2 and 3 the second's.
+    // Each scales its map (by 1 / l, or lambda / l) and hands the other's half over
+    // in its own layout.
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    f32x2 *const meet = (f32x2 *)s_mem + (size_t)wave * kRT * CH * 64 + lane;
+    const f32x2 *const from = (const f32x2 *)s_mem + (size_t)(wave ^ (kWaves / 2)) * kRT * CH * 64 + lane;
+    const DiffParams &d = ar1.p.diff;
+    const int e0 = 2 * map;  // the elements this wave finishes
+    if (active) {
 #pragma unroll
       for (int rt = 0; rt < kRT; ++rt) {
-        f32x4 f;  // lambda / l of row 4j + e
+        f32x4 f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int row = wave_row0 + 16 * rt + 4 * j + e;
           const int tok = q0 + row / G;
-          const bool ok = row < ar1.bq * G && tok < n_new;
-          const float lam =
-              ok ? diff_lambda(ar1.p.diff, qs + tok, kvh * G + row % G) : 0.f;
-          f[e] = lsum[rt][e] > 0.f ? lam / lsum[rt][e] : 0.f;
+          float x = 1.f;
+          if (map == 1)
+            x = row < ar1.bq * G && tok < n_new ? diff_lambda(d, qs + tok, kvh * G + row % G) : 0.f;
+          f[e] = lsum[rt][e] > 0.f ? x / lsum[rt][e] : 0.f;
         }
 #pragma unroll
-        for (int m = 0; m < CH; ++m) meet[(rt * CH + m) * 64] = o[rt][m] * f;
+        for (int m = 0; m < CH; ++m) {
+          o[rt][m] *= f;
+          meet[(rt * CH + m) * 64] =
+              map == 0 ? (f32x2){o[rt][m][2], o[rt][m][3]} : (f32x2){o[rt][m][0], o[rt][m][1]};
+        }
       }
     }
     __syncthreads();
-    if (map == 0 && active) {
-      const DiffParams &d = ar1.p.diff;
+    if (active) {
       float wt[CH];
 #pragma unroll
       for (int m = 0; m < CH; ++m) wt[m] = d.weight != nullptr ? d.weight[16 * m + n16] : 1.f;
 #pragma unroll
       for (int rt = 0; rt < kRT; ++rt) {
-        f32x4 inv, ss = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) inv[e] = lsum[rt][e] > 0.f ? 1.f / lsum[rt][e] : 0.f;
+        f32x2 r[CH], ss = {0.f, 0.f};
 #pragma unroll
         for (int m = 0; m < CH; ++m) {
-          o[rt][m] = o[rt][m] * inv - meet[(rt * CH + m) * 64];
-          ss += o[rt][m] * o[rt][m];
+          const f32x2 other = from[(rt * CH + m) * 64];
+          r[m] = map == 0 ? (f32x2){o[rt][m][0], o[rt][m][1]} - other
+                          : other - (f32x2){o[rt][m][2], o[rt][m][3]};
+          ss += r[m] * r[m];
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < 2; ++e) {
 #pragma unroll
           for (int off = 1; off < 16; off <<= 1) ss[e] += shfl_xor(ss[e], off);
-          const int row = wave_row0 + 16 * rt + 4 * j + e;
+          const int row = wave_row0 + 16 * rt + 4 * j + e0 + e;
           const int tok = q0 + row / G;
           if (row >= ar1.bq * G || tok >= n_new) continue;
           // A row at or past max_query_len (a caller error) is marked with NaN.
@@ -597,7 +627,7 @@ diff_prefill_mfma(const PrefillArgs args) {
           T *dst = (T *)ar1.p.out + (int64_t)(qs + tok) * ar1.p.out_stride_token +
                    (int64_t)(kvh * G + row % G) * ar1.p.out_stride_head + n16;
 #pragma unroll
-          for (int m = 0; m < CH; ++m) dst[16 * m] = (T)(o[rt][m][e] * (f * wt[m]));
+          for (int m = 0; m < CH; ++m) dst[16 * m] = (T)(r[m][e] * (f * wt[m]));
         }
       }
     }
@@ -681,7 +711,7 @@ bool diff_prefill_mfma_covers(const PrefillParams &p, DType dt) {
 
 PrefillSplitShape diff_prefill_split_shape(const PrefillParams &p) {
   const int bk = p.head_dim == 256 ? Shape<256>::kBK : Shape<128>::kBK;
-  return prefill_split_shape(p, pairs_of(p.head_dim), bk, 1, 4, kSplitMinTokens / bk, true);
+  return prefill_split_shape(p, pairs_of(p.head_dim), bk, 1, 1, kSplitMinTokens / bk, true);
 }
 
 hipError_t launch_diff_prefill_mfma(const PrefillParams &p, DType dt, const PrefillSplit *sp,

@@ -56,7 +56,8 @@ inline PrefillSplitShape prefill_split_shape(const PrefillParams &p, int rows, i
   // unsplit, however uneven it is.
   const int64_t entries = (int64_t)p.num_seqs * n_q;
   if (entries > kPrefillSplitItems) return none;
-  // Units are 32-bit on the device (an item's own are at most four tiles').
+  // Units are 32-bit on the device (an item's own are at most six tiles', within the
+  // factor of two that is left).
   if (entries * p.num_kv_heads * (max_tiles + 4) * tile_units >= (int64_t)1 << 30) return none;
   // Chunks of one length that fill whole rounds of the device: over equal cached
   // lengths the 16-bit kernel's natural order (dispatch_slot) makes them even
