@@ -23,7 +23,11 @@
 // latency: a chain of one read of the rows, a scan, a search in LDS, one read of
 // a table or stack entry, one write. Every workgroup scans the rows itself
 // rather than wait for a launch that does, and takes an even share of the step's
-// slots, entries and pushed blocks.
+// slots, entries and pushed blocks. Per launch: 128 rows of one token 4.8 us (5.4
+// a call, which the host bounds); 256 rows that end, wait, grow or come new, 33000
+// slots, 8.0; 512 prompts, a million slots (9 MB), 8.2. Sums in 64 bits cost 0.7 to
+// 1.2 us, a binary search 1 us of the mixed step; workgroups of 512 and 1024
+// threads (fewer scans) ran 9.6 and 11.4 against 9.8 then.
 #include "clover_attn.h"
 #include "clv_device.h"
 
@@ -50,23 +54,34 @@ struct StepTotals {
   int32_t num_free;  // before the step
 };
 
-// Last row whose prefix is <= i (0 <= i < prefix[rows]).
+// Last row whose prefix is <= i (0 <= i < prefix[rows]): three candidates a round,
+// as a round is the latency of its reads.
 __device__ __forceinline__ int row_of(const int32_t *prefix, int rows, int i) {
-  int lo = 0, n = rows;
-  while (n > 1) {
-    const int half = n >> 1;
-    const bool right = prefix[lo + half] <= i;
-    lo += right ? half : 0;
-    n = right ? n - half : half;
+  int lo = 0;
+  for (int n = rows; n > 1;) {
+    n = (n + 3) >> 2;
+    int right = 0;
+#pragma unroll
+    for (int k = 1; k < 4; ++k) right += prefix[min(lo + k * n, rows)] <= i ? 1 : 0;
+    lo += right * n;
   }
   return lo;
+}
+
+// Sums that stay at the largest value instead of wrapping: past every bound
+// that a step is checked against.
+__device__ __forceinline__ uint32_t add_sat(uint32_t a, uint32_t b) {
+  return __builtin_elementwise_add_sat(a, b);
+}
+__device__ __forceinline__ uint32_t clamp32(int64_t x) {
+  return (uint32_t)min(x, (int64_t)0xffffffff);
 }
 
 // Scans the rows into s and checks the step; `write`: also writes the state
 // after it. All NT threads of the workgroup call it.
 template <int NT>
 __device__ StepTotals scan_step(const TablesParams &p, const StepRows &s, bool write) {
-  __shared__ int64_t s_sum[NT / 64][3];
+  __shared__ uint32_t s_sum[NT / 64][3];
   __shared__ int s_flags[NT / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   constexpr int kPer = (CLV_TABLES_MAX_ROWS + NT - 1) / NT;
@@ -90,7 +105,7 @@ __device__ StepTotals scan_step(const TablesParams &p, const StepRows &s, bool w
     return n[k] > 0 ? max((int64_t)held[k], blocks) : (int64_t)held[k];
   };
   // Bit 0: a row longer than its table; bit 1: a state that cannot be.
-  int64_t x[3] = {0, 0, 0};
+  uint32_t x[3] = {0, 0, 0};
   int flags = F < 0 || F > p.num_blocks ? 2 : 0;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) {
@@ -99,17 +114,17 @@ __device__ StepTotals scan_step(const TablesParams &p, const StepRows &s, bool w
     if (len[k] < 0 || held[k] < 0 || held[k] > p.width ||
         len[k] > ((int64_t)held[k] << p.block_shift))
       flags |= 2;
-    x[0] += max(n[k], 0);
-    x[1] += need(k) - held[k];
-    x[2] += n[k] < 0 ? held[k] : 0;
+    x[0] = add_sat(x[0], (uint32_t)max(n[k], 0));
+    x[1] = add_sat(x[1], clamp32(need(k) - held[k]));
+    x[2] = add_sat(x[2], (uint32_t)(n[k] < 0 ? max(held[k], 0) : 0));
   }
-  const int64_t own[3] = {x[0], x[1], x[2]};
+  const uint32_t own[3] = {x[0], x[1], x[2]};
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-      const int64_t y = __shfl_up(x[k], off, 64);
-      if (lane >= off) x[k] += y;
+      const uint32_t y = __shfl_up(x[k], off, 64);
+      if (lane >= off) x[k] = add_sat(x[k], y);
     }
     flags |= __shfl_xor(flags, off, 64);
   }
@@ -119,7 +134,7 @@ __device__ StepTotals scan_step(const TablesParams &p, const StepRows &s, bool w
     s_flags[wave] = flags;
   }
   __syncthreads();
-  int64_t run[3], all[3] = {0, 0, 0};
+  uint32_t run[3], all[3] = {0, 0, 0};  // run: of no use where a sum is at its end
 #pragma unroll
   for (int k = 0; k < 3; ++k) run[k] = x[k] - own[k];
   flags = 0;
@@ -128,15 +143,15 @@ __device__ StepTotals scan_step(const TablesParams &p, const StepRows &s, bool w
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       if (w < wave) run[k] += s_sum[w][k];
-      all[k] += s_sum[w][k];
+      all[k] = add_sat(all[k], s_sum[w][k]);
     }
     flags |= s_flags[w];
   }
   int status = CLV_TABLES_OK;
-  if ((flags & 2) || F + all[2] > p.num_blocks) status = CLV_TABLES_BAD_STATE;
-  else if (all[1] > F + all[2]) status = CLV_TABLES_NO_BLOCKS;
+  if ((flags & 2) || (int64_t)F + all[2] > p.num_blocks) status = CLV_TABLES_BAD_STATE;
+  else if ((int64_t)all[1] > (int64_t)F + all[2]) status = CLV_TABLES_NO_BLOCKS;
   else if (flags & 1) status = CLV_TABLES_ROW_FULL;
-  else if (all[0] > p.num_tokens) status = CLV_TABLES_NO_SLOTS;
+  else if ((int64_t)all[0] > p.num_tokens) status = CLV_TABLES_NO_SLOTS;
   const bool ok = status == CLV_TABLES_OK;
   StepTotals t;
   t.num_free = F;
@@ -160,7 +175,7 @@ __device__ StepTotals scan_step(const TablesParams &p, const StepRows &s, bool w
       p.blocks_held_out[r] = !ok ? held[k] : n[k] < 0 ? 0 : (int32_t)need(k);
     }
     run[0] += max(n[k], 0);
-    run[1] += need(k) - held[k];
+    run[1] += (uint32_t)(need(k) - held[k]);
     run[2] += n[k] < 0 ? held[k] : 0;
   }
   if (tid == 0) {
@@ -261,7 +276,8 @@ __global__ void __launch_bounds__(NT) tables_step(const TablesParams p, bool wri
 
 // In place, the state may only be written when every workgroup has read it:
 // up to this many tokens one workgroup serves the step, above it a second
-// launch writes the state.
+// launch writes the state. One workgroup / two launches, us, 32 rows: 1024 tokens
+// 4.8/6.7, 4096 5.5/6.9, 8192 7.1/7.2, 16384 10.8/7.5; 256 rows the same within 0.8.
 constexpr int64_t kInPlaceTokens = 8192;
 
 }  // namespace

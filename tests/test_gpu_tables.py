@@ -199,3 +199,15 @@ def test_native_argument_block_is_the_python_one(monkeypatch):
         assert real("fill_tables_args", _native.TablesArgs(), *bad, *outs) is None, i
         with pytest.raises((ValueError, RuntimeError)):
             kernels._tables_args(*bad, *outs)
+
+
+@pytest.mark.parametrize("new", [[2 ** 31 - 1, 2 ** 31 - 1, 2], [2 ** 31 - 1] * 130,
+                                 [0, 2 ** 31 - 1] * 700])
+@pytest.mark.parametrize("bs", [1, 16])
+def test_sums_past_32_bits_are_refused(new, bs):
+    """Totals that would wrap to a small number: the step is refused for what
+    it asks (the allocator runs out of blocks), and nothing moves."""
+    s = State(len(new), 4, 50, bs)
+    assert s.step(new, 64, reserve=0) == od.TABLES_NO_BLOCKS
+    assert s.step([1] * min(len(new), 40) + [0] * max(0, len(new) - 40), 64,
+                  in_place=False, reserve=0) == od.TABLES_OK
