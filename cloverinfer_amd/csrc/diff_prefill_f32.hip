@@ -441,7 +441,7 @@ hipError_t launch_td(const PrefillParams &p, const PrefillSplit *sp, hipStream_t
     hipLaunchKernelGGL((diff_prefill_f32<D, true>), dim3((unsigned)sp->groups), dim3(kThreads), 0,
                        stream, args);
     hipLaunchKernelGGL((diff_prefill_merge<float, D, kPairs>),
-                       dim3((unsigned)sp->groups, kPairs / kDiffMergeRows), dim3(256), 0, stream,
+                       dim3((unsigned)sp->groups, kPairs / diff_merge_rows<D>()), dim3(256), 0, stream,
                        args);
     return hipGetLastError();
   }
