@@ -1009,19 +1009,33 @@ int fill_tables(const clv_tables_args *a, clv::TablesParams *p) {
   if (a->rows > 0 && (!a->blocks_held || !a->context_lens || !a->new_lens || !a->blocks_held_out ||
                       !a->context_lens_out || (a->width > 0 && !a->block_tables)))
     return CLV_EINVAL;
-  // An output is its own input or apart from all of them: the state is read by
-  // many workgroups while it is written.
-  const struct {
-    const int32_t *in, *out;
-    int64_t n;
-  } state[4] = {{a->blocks_held, a->blocks_held_out, a->rows},
-                {a->context_lens, a->context_lens_out, a->rows},
-                {a->num_free, a->num_free_out, 1},
-                {a->new_lens, nullptr, a->rows}};
-  for (const auto &o : state)
-    for (const auto &i : state)
-      if (o.out != nullptr && i.in != nullptr && o.out < i.in + i.n && i.in < o.out + o.n &&
-          !(&o == &i && o.out == o.in))
+  // What is written is apart from everything else (a count's output may be its
+  // input): many workgroups read while others write.
+  struct Range {
+    const char *begin, *end;
+    bool written;
+  } range[12];
+  int n = 0;
+  auto add = [&](const void *x, int64_t bytes, bool written) {
+    if (bytes > 0) range[n++] = Range{(const char *)x, (const char *)x + bytes, written};
+  };
+  auto add_state = [&](const int32_t *in, const int32_t *out, int64_t count) {
+    add(in, 4 * count, out == in);
+    if (out != in) add(out, 4 * count, true);
+  };
+  add_state(a->blocks_held, a->blocks_held_out, a->rows);
+  add_state(a->context_lens, a->context_lens_out, a->rows);
+  add_state(a->num_free, a->num_free_out, 1);
+  add(a->new_lens, 4 * (int64_t)a->rows, false);
+  add(a->block_tables, 4 * (int64_t)a->rows * a->width, true);
+  add(a->free_blocks, 4 * (int64_t)a->num_blocks, true);
+  add(a->slot_mapping, 8 * a->num_tokens, true);
+  add(a->query_start_loc, 4 * ((int64_t)a->rows + 1), true);
+  add(a->status, 4, true);
+  for (int i = 0; i < n; ++i)
+    for (int k = 0; k < i; ++k)
+      if ((range[i].written || range[k].written) && range[i].begin < range[k].end &&
+          range[k].begin < range[i].end)
         return CLV_EINVAL;
   *p = clv::TablesParams{a->block_tables,     a->blocks_held,      a->context_lens,
                          a->new_lens,         a->free_blocks,      a->num_free,

@@ -124,17 +124,15 @@ struct DecodeWave {
   static constexpr int KT_ROW = D * EB + 32;
   static constexpr int KT_BYTES = KT ? 16 * KT_ROW : 16;  // 16: no transpose buffer
   static_assert(!KT || (UNI && D >= 128), "K transpose needs block_size >= 16 and whole 256-byte rows");
-  static_assert(!KV8 || KT, "fp8 pools are read on the K-transpose path");
+  static_assert(!KV8 || (KT && D == 128), "fp8 pools are read on the K-transpose path");
   static constexpr int EBC = KV8 ? 1 : EB;  // bytes per cache element
   typedef typename VChunk<CH>::type vchunk_t;
-  typedef uint32_t v8_t __attribute__((ext_vector_type(2 * WORDS)));  // KV8: fp8 chunk of a row
 
   // Loads of one step: K rows (lane row n16) and the V rows 4j..4j+3.
   struct Regs {
     u32x4 k[NQK];
     vchunk_t v[4];
-    u32x2 k8[KV8 ? NQK : 1];  // KV8: the loaded fp8 values
-    v8_t v8[KV8 ? 4 : 1];
+    u32x2 k8[KV8 ? NQK : 1], v8[KV8 ? 4 : 1];  // KV8: the loaded fp8 values
     bool ok;  // the lane's V rows lie in a readable block
   };
 
@@ -238,18 +236,9 @@ struct DecodeWave {
     const rsrc_t rv = make_rsrc(vbase + off);
     if constexpr (KV8) {
 #pragma unroll
-      for (int i = 0; i < NQK; ++i)
-        R.k8[i] = buf_load<u32x2, kCacheStream>(rk, v_lane[i & 3] + (i >> 2) * (D / WORDS));
+      for (int i = 0; i < NQK; ++i) R.k8[i] = buf_load<u32x2, kCacheStream>(rk, v_lane[i]);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if constexpr (WORDS == 1) {
-          R.v8[r] = buf_load<u32x2, kCacheStream>(rv, v_lane[r]);
-        } else {
-          const u32x2 a = buf_load<u32x2, kCacheStream>(rv, v_lane[r]);
-          const u32x2 b = buf_load<u32x2, kCacheStream>(rv, v_lane[r] + D / WORDS);
-          R.v8[r] = __builtin_shufflevector(a, b, 0, 1, 2, 3);
-        }
-      }
+      for (int r = 0; r < 4; ++r) R.v8[r] = buf_load<u32x2, kCacheStream>(rv, v_lane[r]);
       return;
     } else if constexpr (KT) {
 #pragma unroll
@@ -363,7 +352,7 @@ struct DecodeWave {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         if (x[r] == kNegInf) {  // keep NaN/Inf of unused slots out of P.V
-          if constexpr (KV8) R.v8[r] = v8_t{};
+          if constexpr (KV8) R.v8[r] = (u32x2){0u, 0u};
           else R.v[r] = z;
         }
       }

@@ -159,8 +159,9 @@ typedef struct clv_diff_args {
  * rows and then allocate() (reserve = 1) or append_slot() for the growing ones.
  * Written: table entries a row gains, the stack entries pushed and left on it,
  * and the outputs; all else stays as it was (also the entries of rows that
- * ended: columns at or past blocks_held are not part of the table). The _out
- * pointers may be the inputs. All or nothing: where status[0] is not
+ * ended: columns at or past blocks_held are not part of the table). An _out
+ * pointer may be its input; apart from that, what is written must not overlap
+ * anything else (CLV_EINVAL). All or nothing: where status[0] is not
  * CLV_TABLES_OK the state is kept, query_start_loc is 0 and every slot -1.
  */
 enum clv_tables_status {
@@ -450,9 +451,9 @@ size_t clv_prefill_workspace_bytes(const clv_prefill_args *args);
  * Differential decode: clv_paged_decode's call (args: num_heads pairs, head_dim
  * both halves) with the two maps and their joint of clv_diff_args. k_scales and
  * v_scales are null, or the pools are fp8 as in clv_paged_decode_fp8 (head_dim
- * 128, block_size >= 16). Contexts of up to 512 tokens (num_waves <= 0), and
- * shapes that the balanced decode does not take, are one launch without a
- * workspace; the rest is a balanced decode over num_waves waves (<= 0: the
+ * 128, block_size >= 16; at most 4096 segments). Contexts of up to 512 tokens
+ * (num_waves <= 0), and shapes that the balanced decode does not take, are one
+ * launch without a workspace; the rest is a balanced decode over num_waves waves (<= 0: the
  * device default) and its merge. `workspace`: at least
  * clv_diff_decode_workspace_bytes() bytes, 256-byte aligned; may be null where
  * that is 0. A row whose context is empty or unreadable comes out as zeros.

@@ -208,6 +208,14 @@ def test_tables_outputs_that_overlap_inputs(native_lib):
                {"context_lens_out": lens - 4}, {"num_free_out": held + 396}, {"num_free_out": count + 0,
                 "blocks_held_out": count - 8}):
         assert call(**kw) == _native.CLV_EINVAL, kw
+    # what every step writes, on an input, on the state or on each other
+    table, stack, slots, qsl, status = 0x1000, 0x5000, 0xa000, 0xb000, 0xc000
+    for kw in ({"query_start_loc": lens}, {"query_start_loc": new + 396}, {"status": count},
+               {"status": table + 1596}, {"status": qsl + 400}, {"new_lens": stack + 28},
+               {"num_tokens": 4, "slot_mapping": stack + 24},
+               {"num_tokens": 4, "slot_mapping": held - 24}, {"blocks_held_out": table},
+               {"num_tokens": 600, "slot_mapping": slots}, {"num_free_out": status}):
+        assert call(**kw) == _native.CLV_EINVAL, kw
 
 
 def test_struct_layouts(tmp_path):

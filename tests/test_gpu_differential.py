@@ -528,3 +528,8 @@ def test_native_argument_block_is_the_python_one(monkeypatch):
         assert real("fill_diff_args", _native.DiffArgs(), q, x, w, 1e-6, 0.2) is None
         with pytest.raises(ValueError):
             kernels._diff_args(q, x, w, 1e-6, 0.2)
+
+
+def test_decode_more_segments_than_the_split_takes():
+    """Past 4096 segments a workgroup each, at any length."""
+    _decode([3 + (i * 13) % 40 for i in range(1030)] + [700], 4, 4, 64, torch.bfloat16)
