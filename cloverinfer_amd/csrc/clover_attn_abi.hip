@@ -830,8 +830,8 @@ int fill_diff(const clv_diff_args *d, clv::DiffParams *out) {
 
 // Least steps of a group of the balanced differential decode: fewer groups read
 // less each, more of them leave more partials to the merge. Four sequences of
-// 150..3900 tokens, 14/2 heads of 256, bf16: 1 step 25.5 us, 2 20.6, 4 19.5,
-// 8 22.7, 16 31.5; full batches have more steps a group than this anyway.
+// 150..3900 tokens, 14/2 heads of 256, bf16, balanced: 1 step 25.5 us, 2 20.6, 4
+// 19.5, 8 22.7, 16 31.5; full batches have more steps a group than this anyway.
 constexpr int32_t kDiffMinSteps = 4;
 
 // `a` with the rows of both maps as its heads.
@@ -842,6 +842,47 @@ int diff_rows(const clv_decode_args *a, clv_decode_args *rows) {
   *rows = *a;
   rows->num_heads = 2 * a->num_heads;
   return CLV_OK;
+}
+
+// Segments (sequence x kv head x 16 rows) of a differential decode.
+int64_t diff_segments(const clv_decode_args &rows) {
+  return (int64_t)rows.num_seqs * rows.num_kv_heads *
+         ceil_div(rows.num_heads / rows.num_kv_heads, 16);
+}
+
+// Small batches: the tokens of every segment in partitions of a multiple of 64, a
+// workgroup of four waves each, about kDiffGrid of them. Against the balanced
+// decode there is no scan before the first load, and four waves share a partial.
+// Partitions / balanced, us, contexts of 0.25..1 of the bound:
+//                           1000        4000        16000
+//   2 seqs, 14/2 x 256 bf16 12.2/17.3   13.7/18.3   16.5/25.6
+//   8 seqs                  12.9/17.6   16.7/21.7   39.7/43.4
+//   32 seqs                 16.8/21.1   37.5/42.0   119/113
+//   4 seqs, 28/4 x 128 bf16 11.0/14.8   12.4/17.0   27.7/31.7
+//   32 seqs                 17.6/21.6   43.5/40.7   165/115
+//   4 seqs, 6/6 x 128 fp32  11.9/18.2   14.9/18.9   48.5/47.0
+//   16 seqs                 21.3/18.8   54.2/41.4   233/167
+// so where the pools' rows up to the bound are at most kDiffGridBytes and the
+// segments at most kDiffGridSegments (fp32: half). With 512 workgroups 256-wide heads
+// lose (8 x 4000 21.7, two are resident on a unit), 64-wide ones win (8 x 16000
+// 24.8, with 256 34.3, balanced 28.2); smallest partitions of 128 equal those of 64.
+constexpr int64_t kDiffGrid = 256;
+constexpr int64_t kDiffGridBytes = 200 << 20;
+constexpr int64_t kDiffGridSegments = 128;
+
+// Tokens of a partition, 0: no partitions.
+int32_t diff_partition(const clv_decode_args &rows, bool fp8, int32_t num_waves) {
+  if (fp8 || num_waves > 0 || rows.num_seqs <= 0 ||
+      !clv::diff_decode_mfma_supported(rows.head_dim, rows.block_size))
+    return 0;
+  const int64_t segments = diff_segments(rows), eb = elem_bytes(rows.dtype);
+  if (segments * eb > 2 * kDiffGridSegments ||
+      2 * eb * rows.head_dim * rows.num_kv_heads * rows.num_seqs * rows.max_context_len >
+          kDiffGridBytes)
+    return 0;
+  const int64_t grid = rows.head_dim == 64 ? 2 * kDiffGrid : kDiffGrid;
+  const int64_t parts = std::max<int64_t>(1, grid / segments);
+  return (int32_t)(std::max<int64_t>(1, ceil_div(ceil_div(rows.max_context_len, parts), 64)) * 64);
 }
 
 // Longest context for which a differential decode runs as one launch, a
@@ -855,7 +896,10 @@ int diff_rows(const clv_decode_args *a, clv_decode_args *rows) {
 //   128 seqs, 14/2 x 256 bf16    9.5/21.6   25.2/37.5  43.6/57.0  81.3/95.8
 // Past it one launch would still win for many sequences of one length, but it
 // takes as long as its longest sequence, which a ragged batch (what decodes
-// there) has alone.
+// there) has alone. Where partitions are the other choice, key rows of 512 bytes
+// or more take half of it: one launch / partitions of 8 x 256, 320 and 512 tokens
+// 11.0/11.2, 12.4/11.4, 16.1/11.8 us (14/2 x 256 bf16), narrower ones 8.5/11.4,
+// 9.4/11.5, 11.6/11.2 (28/4 x 128 bf16).
 constexpr int32_t kDiffSinglePassMaxLen = 512;
 
 // Most segments (sequence x kv head x 16 rows) of head_dim 256 that take it. Two
@@ -869,9 +913,12 @@ constexpr int64_t kDiffSinglePassWideSegments = 512;
 bool diff_single_pass(const clv_decode_args &rows, bool fp8, int32_t num_waves) {
   if (fp8) return false;
   if (!clv::diff_decode_mfma_supported(rows.head_dim, rows.block_size)) return true;
-  const int64_t segments = (int64_t)rows.num_seqs * rows.num_kv_heads *
-                           ceil_div(rows.num_heads / rows.num_kv_heads, 16);
-  if (num_waves <= 0 && rows.max_context_len <= kDiffSinglePassMaxLen &&
+  const int64_t segments = diff_segments(rows);
+  const bool wide = rows.head_dim * elem_bytes(rows.dtype) >= 512;
+  const int32_t max_len = wide && diff_partition(rows, fp8, num_waves) > 0
+                              ? kDiffSinglePassMaxLen / 2
+                              : kDiffSinglePassMaxLen;
+  if (num_waves <= 0 && rows.max_context_len <= max_len &&
       (rows.head_dim <= 128 || segments <= kDiffSinglePassWideSegments))
     return true;
   // More segments than the balanced decode takes: a workgroup each fills the chip.
@@ -904,6 +951,8 @@ extern "C" {
 size_t clv_diff_decode_workspace_bytes(const clv_decode_args *a, int32_t fp8, int32_t num_waves) {
   clv_decode_args r;
   if (diff_rows(a, &r) != CLV_OK || diff_single_pass(r, fp8 != 0, num_waves)) return 0;
+  if (const int32_t size = diff_partition(r, fp8 != 0, num_waves))
+    return clv_splitk_workspace_bytes(r.num_seqs, r.num_heads, r.head_dim, r.max_context_len, size);
   return clv_balanced_workspace_bytes(r.num_seqs, r.num_heads, r.num_kv_heads, r.head_dim,
                                       diff_waves(fp8 != 0, num_waves));
 }
@@ -936,6 +985,16 @@ int clv_diff_decode(const clv_decode_args *a, const clv_diff_args *d, const floa
                                ? clv::launch_diff_decode_mfma(p, dt, s)
                                : clv::launch_diff_decode_valu(p, dt, s);
     return err == hipSuccess ? CLV_OK : CLV_ELAUNCH;
+  }
+  if (const int32_t size = diff_partition(r, fp8, num_waves)) {
+    st = fill_decode(&r, &p);
+    if (st != CLV_OK || p.num_seqs == 0) return st;
+    if ((int64_t)p.num_kv_heads * p.n_gchunks > 65535) return CLV_EUNSUPPORTED;  // grid y limit
+    st = fill_splitk(&r, size, workspace, workspace_bytes, &p);
+    if (st != CLV_OK) return st;
+    p.diff = diff;
+    if (clv::launch_diff_decode_mfma(p, dt, s) != hipSuccess) return CLV_ELAUNCH;
+    return clv::launch_diff_stream_reduce(p, dt, s) == hipSuccess ? CLV_OK : CLV_ELAUNCH;
   }
   st = fill_balanced(&r, diff_waves(fp8, num_waves), workspace, workspace_bytes, &p, true);
   if (st != CLV_OK || p.num_seqs == 0) return st;

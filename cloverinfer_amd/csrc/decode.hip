@@ -82,13 +82,13 @@ __device__ __forceinline__ T *diff_out(const DecodeParams &p, int s, int r0) {
 // so that the rows of a token for HG adjacent kv heads are read together (one
 // contiguous range of the token's row in the pools).
 //
-// DIFF (single pass): differential attention, the rows of both maps (DiffRows),
-// joined where the waves' partials are merged.
+// DIFF: differential attention, the rows of both maps (DiffRows), joined where the
+// waves' partials are merged; with partitions, by diff_stream_reduce.
 template <typename T, int D, int NW, bool UNI, bool APPEND = false, int HG = 1, bool DIFF = false>
 __global__ void __launch_bounds__(NW * HG * 64)
 paged_decode_mfma(const DecodeParams p, const int32_t *__restrict__ tables) {
   static_assert(HG == 1 || (NW == 1 && !APPEND), "head groups: one wave per kv head");
-  static_assert(!DIFF || (HG == 1 && !APPEND), "differential decode: one pass over the pools");
+  static_assert(!DIFF || (HG == 1 && !APPEND), "differential decode: no append, one kv head");
   typedef typename WaveRows<typename GridWave<T, D, UNI>::type, DIFF>::type W;
   __shared__ WaveSmem<NW, 16, D> sms[HG];
 
@@ -198,7 +198,7 @@ paged_decode_mfma(const DecodeParams p, const int32_t *__restrict__ tables) {
     }
   }
   __syncthreads();
-  if constexpr (DIFF)
+  if (DIFF && p.partition_size == 0)
     diff_merge_and_store<T, NW, 16, D>(sm, ng, p.diff, s, h0 / 2, diff_out<T>(p, s, h0),
                                        p.out_stride_head);
   else
@@ -341,10 +341,11 @@ hipError_t launch_valu_t(const DecodeParams &p, hipStream_t stream) {
   }
 }
 
-// Differential decode, one workgroup per (sequence, kv head, 16-row chunk).
+// Differential decode, one workgroup per (sequence, kv head, 16-row chunk) and
+// partition.
 template <typename T, int D>
 hipError_t launch_diff_mfma_td(const DecodeParams &p, hipStream_t stream) {
-  const dim3 grid(1u, (unsigned)(p.num_kv_heads * p.n_gchunks), (unsigned)p.num_seqs);
+  const dim3 grid(p.partition_size > 0 ? (unsigned)p.max_parts : 1u, (unsigned)(p.num_kv_heads * p.n_gchunks), (unsigned)p.num_seqs);
   if (p.block_shift >= 4)
     hipLaunchKernelGGL((paged_decode_mfma<T, D, 4, true, false, 1, true>), grid, dim3(256), 0,
                        stream, p, p.block_tables);
@@ -443,7 +444,7 @@ bool diff_decode_mfma_supported(int head_dim, int block_size) {
 }
 
 hipError_t launch_diff_decode_mfma(const DecodeParams &p, DType dt, hipStream_t stream) {
-  if (p.partition_size != 0 || p.kv_fp8) return hipErrorInvalidValue;
+  if (p.kv_fp8) return hipErrorInvalidValue;
   if (dt == DType::BF16) return launch_diff_mfma_t<__bf16>(p, stream);
   if (dt == DType::F16) return launch_diff_mfma_t<_Float16>(p, stream);
   if (dt == DType::F32) return launch_diff_mfma_t<float>(p, stream);

@@ -554,7 +554,8 @@ __global__ void __launch_bounds__(NW > 1 ? NW * 64 : 256) stream_reduce(const De
 // writes it. A workgroup holds two pairs at NW = 1, one otherwise. The rule is
 // lse_merge's; a lane holds D / 64 consecutive columns, so a row is one load
 // instruction, and the first R rows are loaded with the row maxima and sums.
-template <typename T, int D, int NW>
+// PART: the partials are those of partitions, [sequence, row, partition].
+template <typename T, int D, int NW, bool PART>
 __global__ void __launch_bounds__(NW > 1 ? 2 * NW * 64 : 256)
 diff_stream_reduce(const DecodeParams p) {
   constexpr int EPL = D / 64;
@@ -575,8 +576,15 @@ diff_stream_reduce(const DecodeParams p) {
   const int h = any ? (int)(idx - (int64_t)s * heads) : 0;
   const int kvh = h / (p.group / 2);
   int n;
-  const int64_t row0 = row_partials<true>(p, s, kvh, 2 * h - kvh * p.group + map, n);
-  const int64_t rs = 16 * p.head_group;  // rows between a row's partials
+  int64_t row0, rs;  // the row's first partial, and rows from one to the next
+  if constexpr (PART) {
+    n = (clamp_ctx(p, s) + p.partition_size - 1) / p.partition_size;
+    row0 = ((int64_t)s * p.num_heads + 2 * h + map) * p.max_parts;
+    rs = 1;
+  } else {
+    row0 = row_partials<true>(p, s, kvh, 2 * h - kvh * p.group + map, n);
+    rs = 16 * p.head_group;
+  }
   const float *m = p.ws_m + row0, *l = p.ws_l + row0, *c = p.ws_o + row0 * D + lane * EPL;
   // Wave wv takes chunks of C partials; each lane weighs one of a chunk.
   const int C = NW > 1 ? max(1, min(64, (n + NW - 1) / NW)) : 64;
@@ -786,17 +794,25 @@ hipError_t launch_diff_stream_t(const DecodeParams &p, hipStream_t stream) {
   }
 }
 
-template <typename T, int D>
-hipError_t launch_diff_sreduce_td(const DecodeParams &p, hipStream_t stream) {
+template <typename T, int D, bool PART>
+hipError_t launch_diff_sreduce_tdp(const DecodeParams &p, hipStream_t stream) {
   const int64_t pairs = (int64_t)p.num_seqs * (p.num_heads / 2);
-  const int64_t groups = p.num_waves / p.head_group;
-  if (groups > (int64_t)kWideMergePartials * p.num_segments)
-    hipLaunchKernelGGL((diff_stream_reduce<T, D, kMergeWaves>), dim3((unsigned)pairs),
+  const bool wide = PART ? p.max_parts > kWideMergePartials
+                         : p.num_waves / p.head_group >
+                               (int64_t)kWideMergePartials * p.num_segments;
+  if (wide)
+    hipLaunchKernelGGL((diff_stream_reduce<T, D, kMergeWaves, PART>), dim3((unsigned)pairs),
                        dim3(2 * kMergeWaves * 64), 0, stream, p);
   else
-    hipLaunchKernelGGL((diff_stream_reduce<T, D, 1>), dim3((unsigned)((pairs + 1) / 2)), dim3(256),
-                       0, stream, p);
+    hipLaunchKernelGGL((diff_stream_reduce<T, D, 1, PART>), dim3((unsigned)((pairs + 1) / 2)),
+                       dim3(256), 0, stream, p);
   return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_diff_sreduce_td(const DecodeParams &p, hipStream_t stream) {
+  return p.partition_size > 0 ? launch_diff_sreduce_tdp<T, D, true>(p, stream)
+                              : launch_diff_sreduce_tdp<T, D, false>(p, stream);
 }
 
 template <typename T>

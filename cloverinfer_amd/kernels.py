@@ -818,9 +818,10 @@ def differential_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Te
     arguments are :func:`paged_attention`'s, pools, tables and appends too;
     fp8 pools need head_dim 128 and block_size >= 16. Key values must be finite.
 
-    Contexts of up to 512 tokens are one launch; longer ones (head_dim 64, 128
-    or 256, block_size >= 4) are split evenly over the chip, over ``num_waves``
-    waves (0 = the device default), and joined.
+    Short contexts (up to 256 or 512 tokens) are one launch; longer ones
+    (head_dim 64, 128 or 256, block_size >= 4) are cut into partitions in small
+    batches, split evenly over the chip in large ones, and joined. ``num_waves``
+    > 0 asks for the even split over that many waves at any length.
     """
     a = _decode_args(out, q, k_cache, v_cache, block_tables, context_lens, block_size,
                      max_context_len, _half_scale(scale, q))

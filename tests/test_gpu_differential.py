@@ -533,3 +533,16 @@ def test_native_argument_block_is_the_python_one(monkeypatch):
 def test_decode_more_segments_than_the_split_takes():
     """Past 4096 segments a workgroup each, at any length."""
     _decode([3 + (i * 13) % 40 for i in range(1030)] + [700], 4, 4, 64, torch.bfloat16)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(14, 2, 256, torch.bfloat16), (28, 4, 128, torch.float16),
+                                            (6, 6, 128, torch.float32), (16, 4, 64, torch.bfloat16)])
+@pytest.mark.parametrize("num_waves", [0, 48])  # partitions of a small batch; the even split
+@pytest.mark.parametrize("form", ["ends", "hole", "strided", "bound", "one"])
+def test_decode_splits(hq, hkv, d, dtype, num_waves, form):
+    """Both ways of splitting a small batch: contexts that end on and beside a
+    partition, unreadable blocks, strided rows, lengths past the bound."""
+    ctx = {"ends": [64, 63, 65, 128, 127, 129, 0, 1, 192, 1025], "hole": [1000, 600, 40, 7],
+           "strided": [40, 7, 1300], "bound": [3000, 20, 700], "one": [2111]}[form]
+    _decode(ctx, hq, hkv, d, dtype, num_waves=num_waves, hole=-1 if form == "hole" else None,
+            strided=form == "strided", max_len=900 if form == "bound" else None, lam="row")
