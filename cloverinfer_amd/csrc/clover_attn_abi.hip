@@ -866,21 +866,25 @@ int64_t diff_segments(const clv_decode_args &rows) {
 // segments at most kDiffGridSegments (fp32: half). With 512 workgroups 256-wide heads
 // lose (8 x 4000 21.7, two are resident on a unit), 64-wide ones win (8 x 16000
 // 24.8, with 256 34.3, balanced 28.2); smallest partitions of 128 equal those of 64.
-constexpr int64_t kDiffGrid = 256;
-constexpr int64_t kDiffGridBytes = 200 << 20;
-constexpr int64_t kDiffGridSegments = 128;
+// fp8 pools, whose steps are bound by their vector work, want three workgroups a
+// unit, and gain up to 256 segments and 256 MiB: 16 seqs of up to 4000 tokens, 28/4
+// heads, 256 workgroups 26.6, 512 20.3, 768 20.0, 1024 23.4, balanced 31.9; 64 seqs of
+// up to 4000 41.1/46.5, 100 85/61; 16 of up to 16000, 32/8, 69.4/65.9.
+constexpr int64_t kDiffGrid = 256, kDiffGridFp8 = 768;
+constexpr int64_t kDiffGridBytes = 200 << 20, kDiffGridBytesFp8 = 256 << 20;
+constexpr int64_t kDiffGridSegments = 128, kDiffGridSegmentsFp8 = 256;
 
 // Tokens of a partition, 0: no partitions.
 int32_t diff_partition(const clv_decode_args &rows, bool fp8, int32_t num_waves) {
-  if (fp8 || num_waves > 0 || rows.num_seqs <= 0 ||
+  if (num_waves > 0 || rows.num_seqs <= 0 ||
       !clv::diff_decode_mfma_supported(rows.head_dim, rows.block_size))
     return 0;
-  const int64_t segments = diff_segments(rows), eb = elem_bytes(rows.dtype);
-  if (segments * eb > 2 * kDiffGridSegments ||
+  const int64_t segments = diff_segments(rows), eb = fp8 ? 1 : elem_bytes(rows.dtype);
+  if (segments * eb > (fp8 ? kDiffGridSegmentsFp8 : 2 * kDiffGridSegments) ||
       2 * eb * rows.head_dim * rows.num_kv_heads * rows.num_seqs * rows.max_context_len >
-          kDiffGridBytes)
+          (fp8 ? kDiffGridBytesFp8 : kDiffGridBytes))
     return 0;
-  const int64_t grid = rows.head_dim == 64 ? 2 * kDiffGrid : kDiffGrid;
+  const int64_t grid = fp8 ? kDiffGridFp8 : rows.head_dim == 64 ? 2 * kDiffGrid : kDiffGrid;
   const int64_t parts = std::max<int64_t>(1, grid / segments);
   return (int32_t)(std::max<int64_t>(1, ceil_div(ceil_div(rows.max_context_len, parts), 64)) * 64);
 }
@@ -911,10 +915,9 @@ constexpr int32_t kDiffSinglePassMaxLen = 512;
 constexpr int64_t kDiffSinglePassWideSegments = 512;
 
 bool diff_single_pass(const clv_decode_args &rows, bool fp8, int32_t num_waves) {
-  if (fp8) return false;
   if (!clv::diff_decode_mfma_supported(rows.head_dim, rows.block_size)) return true;
   const int64_t segments = diff_segments(rows);
-  const bool wide = rows.head_dim * elem_bytes(rows.dtype) >= 512;
+  const bool wide = !fp8 && rows.head_dim * elem_bytes(rows.dtype) >= 512;
   const int32_t max_len = wide && diff_partition(rows, fp8, num_waves) > 0
                               ? kDiffSinglePassMaxLen / 2
                               : kDiffSinglePassMaxLen;
@@ -976,11 +979,18 @@ int clv_diff_decode(const clv_decode_args *a, const clv_diff_args *d, const floa
   const hipStream_t s = (hipStream_t)stream;
   const DType dt = (DType)a->dtype;
   clv::DecodeParams p;
+  auto set_own = [&] {  // what the fills of plain decode do not know
+    p.diff = diff;
+    p.stream_min_steps = kDiffMinSteps;
+    p.kv_fp8 = fp8 ? 1 : 0;
+    p.k_scales = k_scales;
+    p.v_scales = v_scales;
+  };
   if (diff_single_pass(r, fp8, num_waves)) {
     st = fill_decode(&r, &p);
     if (st != CLV_OK || p.num_seqs == 0) return st;
     if ((int64_t)p.num_kv_heads * p.n_gchunks > 65535) return CLV_EUNSUPPORTED;  // grid y limit
-    p.diff = diff;
+    set_own();
     const hipError_t err = clv::diff_decode_mfma_supported(a->head_dim, a->block_size)
                                ? clv::launch_diff_decode_mfma(p, dt, s)
                                : clv::launch_diff_decode_valu(p, dt, s);
@@ -992,19 +1002,13 @@ int clv_diff_decode(const clv_decode_args *a, const clv_diff_args *d, const floa
     if ((int64_t)p.num_kv_heads * p.n_gchunks > 65535) return CLV_EUNSUPPORTED;  // grid y limit
     st = fill_splitk(&r, size, workspace, workspace_bytes, &p);
     if (st != CLV_OK) return st;
-    p.diff = diff;
+    set_own();
     if (clv::launch_diff_decode_mfma(p, dt, s) != hipSuccess) return CLV_ELAUNCH;
     return clv::launch_diff_stream_reduce(p, dt, s) == hipSuccess ? CLV_OK : CLV_ELAUNCH;
   }
   st = fill_balanced(&r, diff_waves(fp8, num_waves), workspace, workspace_bytes, &p, true);
   if (st != CLV_OK || p.num_seqs == 0) return st;
-  p.diff = diff;
-  p.stream_min_steps = kDiffMinSteps;
-  if (fp8) {
-    p.kv_fp8 = 1;
-    p.k_scales = k_scales;
-    p.v_scales = v_scales;
-  }
+  set_own();
   if (clv::launch_diff_decode_stream(p, dt, s) != hipSuccess) return CLV_ELAUNCH;
   return clv::launch_diff_stream_reduce(p, dt, s) == hipSuccess ? CLV_OK : CLV_ELAUNCH;
 }

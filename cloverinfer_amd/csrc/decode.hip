@@ -27,6 +27,8 @@
 // decomposition and the same epilogue.
 #include "decode_mfma.h"
 
+#include <type_traits>
+
 namespace clv {
 namespace {
 
@@ -84,12 +86,16 @@ __device__ __forceinline__ T *diff_out(const DecodeParams &p, int s, int r0) {
 //
 // DIFF: differential attention, the rows of both maps (DiffRows), joined where the
 // waves' partials are merged; with partitions, by diff_stream_reduce.
-template <typename T, int D, int NW, bool UNI, bool APPEND = false, int HG = 1, bool DIFF = false>
+// KV8 (DIFF, 16-bit T): fp8 pools, read on the K-transpose path (DecodeWave).
+template <typename T, int D, int NW, bool UNI, bool APPEND = false, int HG = 1, bool DIFF = false,
+          bool KV8 = false>
 __global__ void __launch_bounds__(NW * HG * 64)
 paged_decode_mfma(const DecodeParams p, const int32_t *__restrict__ tables) {
   static_assert(HG == 1 || (NW == 1 && !APPEND), "head groups: one wave per kv head");
   static_assert(!DIFF || (HG == 1 && !APPEND), "differential decode: no append, one kv head");
-  typedef typename WaveRows<typename GridWave<T, D, UNI>::type, DIFF>::type W;
+  static_assert(!KV8 || DIFF, "plain decode over fp8 pools: the balanced kernel");
+  typedef typename std::conditional<KV8, StreamWave<T, D, UNI, KV8>, GridWave<T, D, UNI>>::type Wave;
+  typedef typename WaveRows<typename Wave::type, DIFF>::type W;
   __shared__ WaveSmem<NW, 16, D> sms[HG];
 
   const int hw = HG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
@@ -134,9 +140,16 @@ paged_decode_mfma(const DecodeParams p, const int32_t *__restrict__ tables) {
 
   W w;
   w.init(p);
+  float out_scale = 1.f;  // of the accumulators: the value scale of fp8 pools
+  if constexpr (KV8) {
+    __shared__ __attribute__((aligned(16))) char s_kt[NW][W::KT_BYTES];
+    w.set_k_lds(s_kt[wave]);
+    out_scale = p.v_scales[kvh];
+    w.set_kv_scales(p.scale_log2 * p.k_scales[kvh], out_scale);
+  }
   typename W::qk_t qop[W::NQK];
   w.load_q(p, s, h0, ng, qop);
-  const SegGeom geo = seg_geom<T>(p, s, kvh, t_end, tables);
+  const SegGeom geo = seg_geom<T, KV8 ? 1 : (int)sizeof(T)>(p, s, kvh, t_end, tables);
 
   // The prefetch is unconditional (a branch around it makes the compiler wait
   // for every outstanding load): past the wave's last step it re-reads that
@@ -194,6 +207,7 @@ paged_decode_mfma(const DecodeParams p, const int32_t *__restrict__ tables) {
 #pragma unroll
     for (int m = 0; m < W::CH; m += 4) {
       f32x4 v = {w.o[m][r], w.o[m + 1][r], w.o[m + 2][r], w.o[m + 3][r]};
+      if constexpr (KV8) v *= out_scale;
       store_vec<f32x4>(dst + W::col_of(w.n16, m), v);
     }
   }
@@ -357,6 +371,17 @@ hipError_t launch_diff_mfma_td(const DecodeParams &p, hipStream_t stream) {
 
 template <typename T>
 hipError_t launch_diff_mfma_t(const DecodeParams &p, hipStream_t stream) {
+  if (p.kv_fp8) {
+    if constexpr (sizeof(T) == 2) {
+      if (p.head_dim != 128 || p.block_shift < 4) return hipErrorInvalidValue;
+      const dim3 grid(p.partition_size > 0 ? (unsigned)p.max_parts : 1u,
+                      (unsigned)(p.num_kv_heads * p.n_gchunks), (unsigned)p.num_seqs);
+      hipLaunchKernelGGL((paged_decode_mfma<T, 128, 4, true, false, 1, true, true>), grid, dim3(256),
+                         0, stream, p, p.block_tables);
+      return hipGetLastError();
+    }
+    return hipErrorInvalidValue;
+  }
   switch (p.head_dim) {
     case 64: return launch_diff_mfma_td<T, 64>(p, stream);
     case 128: return launch_diff_mfma_td<T, 128>(p, stream);
@@ -444,7 +469,6 @@ bool diff_decode_mfma_supported(int head_dim, int block_size) {
 }
 
 hipError_t launch_diff_decode_mfma(const DecodeParams &p, DType dt, hipStream_t stream) {
-  if (p.kv_fp8) return hipErrorInvalidValue;
   if (dt == DType::BF16) return launch_diff_mfma_t<__bf16>(p, stream);
   if (dt == DType::F16) return launch_diff_mfma_t<_Float16>(p, stream);
   if (dt == DType::F32) return launch_diff_mfma_t<float>(p, stream);

@@ -451,7 +451,7 @@ size_t clv_prefill_workspace_bytes(const clv_prefill_args *args);
  * Differential decode: clv_paged_decode's call (args: num_heads pairs, head_dim
  * both halves) with the two maps and their joint of clv_diff_args. k_scales and
  * v_scales are null, or the pools are fp8 as in clv_paged_decode_fp8 (head_dim
- * 128, block_size >= 16; at most 4096 segments). num_waves > 0: a balanced decode
+ * 128, block_size >= 16). num_waves > 0: a balanced decode
  * over that many waves, and its merge. num_waves <= 0 chooses: one launch without a
  * workspace for contexts of up to 512 tokens (256 where it pays to split them), and
  * for shapes that the others do not take; partitions and their merge for small

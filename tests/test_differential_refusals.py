@@ -154,7 +154,9 @@ def test_decode_arguments(native_lib):
     assert call(a, _diff()) == _native.CLV_EWORKSPACE
     a.max_context_len = 512
     assert native_lib.clv_diff_decode_workspace_bytes(a, 0, 0) == 0
-    assert native_lib.clv_diff_decode_workspace_bytes(a, 1, 0) > 0
+    assert native_lib.clv_diff_decode_workspace_bytes(a, 1, 0) == 0
+    assert native_lib.clv_diff_decode_workspace_bytes(a, 0, 64) > 0
+    assert native_lib.clv_diff_decode_workspace_bytes(a, 1, 64) > 0
     a.num_heads = 30
     assert call(a, _diff()) == _native.CLV_EINVAL
 

@@ -187,9 +187,10 @@ def test_decode_equal_maps_cancel(kind):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("hq,hkv", [(28, 4), (6, 6), (24, 2)])
 @pytest.mark.parametrize("ctx", [[1, 0, 17, 400], [3000, 1, 700]])
-def test_decode_fp8_pools(dtype, hq, hkv, ctx):
+@pytest.mark.parametrize("num_waves", [0, 48])  # one launch or partitions; the even split
+def test_decode_fp8_pools(dtype, hq, hkv, ctx, num_waves):
     d, bs, n = 128, 16, len(ctx)
-    print(f"differential decode fp8 {dtype} {hq}/{hkv} ctx {ctx}", flush=True)
+    print(f"differential decode fp8 {dtype} {hq}/{hkv} ctx {ctx} waves {num_waves}", flush=True)
     k, v, tables = make_paged_kv(5, ctx, hkv, d, bs, dtype)
     g = torch.Generator().manual_seed(6)
     ks, vs = (torch.rand(hkv, generator=g) * 0.02 + 0.01 for _ in range(2))
@@ -205,7 +206,8 @@ def test_decode_fp8_pools(dtype, hq, hkv, ctx):
     out = torch.full((n, hq, d), float("nan"), dtype=dtype, device=DEV)
     kernels.differential_attention(out, q.to(DEV), k8, v8, padded_tables(tables).to(DEV),
                                    torch.tensor(ctx, dtype=torch.int32, device=DEV), bs, max(ctx),
-                                   0.6, norm_weight=weight.to(DEV), k_scale=ks, v_scale=vs.to(DEV))
+                                   0.6, norm_weight=weight.to(DEV), k_scale=ks, v_scale=vs.to(DEV),
+                                   num_waves=num_waves)
     for s in range(n):
         ref = od.rows(q[s:s + 1], _gathered(kd, tables[s], ctx[s], bs),
                       _gathered(vd, tables[s], ctx[s], bs), [ctx[s]], 0.6, weight)
