@@ -95,10 +95,14 @@ template <int D> struct SplitCfg {
   }
 };
 
-// Table width in tokens up to which a call is not split (91 batches of 1..1024
-// tokens, sum: 128 3701 us, 256 3665, 512 3451, 1024 3322; 91 of up to 5000 tokens:
-// 1024 7291, 1536 7425, 2048 8087, 4096 10130).
-constexpr int kSplitMinTokens = 1024;
+// Table width in tokens up to which a call is not split. Items (counted at the
+// longest chunk) of up to 9/4 rounds of the device: a cut costs what the evenness
+// gives (one prompt of 777 tokens, 16/16 x 256, 35.7 us unsplit and 51.5 split; three
+// of 488..663, 528 items, 54 and 60). More of them run long after the others end:
+// eight prompts of 17..1000 tokens, 32/8 x 128, 2048 items, 168 and 105; 16 of 30..500
+// 142 and 102; 24 of up to 200 behind 700, 16/16 x 256, 121 and 62; five of 285..999,
+// 28/4 x 128, 104 and 91.
+constexpr int kSplitMinTokens = 1024, kSplitMinTokensMany = 256;
 
 // Eight values of V (token `pos`, columns d0 ..) with 0 in the place of NaN and
 // infinities; seen_by[column] remembers the first token with a NaN there,
@@ -711,7 +715,11 @@ bool diff_prefill_mfma_covers(const PrefillParams &p, DType dt) {
 
 PrefillSplitShape diff_prefill_split_shape(const PrefillParams &p) {
   const int bk = p.head_dim == 256 ? Shape<256>::kBK : Shape<128>::kBK;
-  return prefill_split_shape(p, pairs_of(p.head_dim), bk, 1, 1, kSplitMinTokens / bk, true);
+  const int64_t bq = max(1, pairs_of(p.head_dim) / p.group);
+  const int64_t items = (p.max_query_len + bq - 1) / bq * p.num_seqs * p.num_kv_heads;
+  const bool many = 4 * items > 9 * 8 * (int64_t)p.cus_per_xcd;
+  return prefill_split_shape(p, pairs_of(p.head_dim), bk, 1, 1,
+                             (many ? kSplitMinTokensMany : kSplitMinTokens) / bk, true);
 }
 
 hipError_t launch_diff_prefill_mfma(const PrefillParams &p, DType dt, const PrefillSplit *sp,
